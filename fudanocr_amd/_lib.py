@@ -115,6 +115,12 @@ SIGNATURES = {
     "focr_l1_masked_fwd": [P, P, P, P, L, I, I, P, P],
     "focr_l1_masked_bwd": [P, P, P, P, L, I, I, P, P],
     "focr_weight_cross_entropy_masked_fwd": [P, P, P, P, P, P, L, I, P, P],
+    "focr_paged_append": [P, P, L, L, L, L, P, P, P, P, P, L, I, I, I, I, I, L, I, P],
+    "focr_paged_attention_ws_bytes": [L, I, I, I, I, I, I, I],
+    "focr_paged_attention_fwd": [P, L, L, P, P, P, P, P, P, L, L, P, L, L, I, I, I, I, I, I, L, I, I, F, I, I, P],
+    "focr_beam_select_ws_bytes": [I, I, I, I, I],
+    "focr_beam_select": [P, L, L, P, P, P, P, P, P, P, L, I, I, I, I, I, I, P],
+    "focr_beam_reorder": [P, P, P, P, P, P, P, I, I, I, I, I, I, I, L, I, P],
     "focr_set_precision": [I],
     "focr_set_tuning": [I, I],
     "focr_comm_unique_id": [P],
@@ -181,6 +187,8 @@ def load():
     lib.focr_weight_frag_bytes.restype = ctypes.c_long
     lib.focr_psnr_ssim_ws_floats.restype = ctypes.c_long
     lib.focr_fe_wgrads_ws_floats.restype = ctypes.c_long
+    lib.focr_paged_attention_ws_bytes.restype = ctypes.c_long
+    lib.focr_beam_select_ws_bytes.restype = ctypes.c_long
     lib.focr_attention_keep_scale.restype = ctypes.c_float
     _lib = lib
     if os.environ.get("FOCR_PRECISION"):          # 0 fp32 | 1 bf16x3 | 2 (default) + bf16 attention-gradient sums | 3 + bf16 dgrad

@@ -11,6 +11,10 @@
 #define FOCR_EHIP (-3)
 #define FOCR_ENCCL (-4)
 
+#define FOCR_DT_F32 0
+#define FOCR_DT_BF16 1
+#define FOCR_DT_F16 2
+
 extern "C" void focr_set_error(const char* fmt, ...);
 extern "C" int focr_get_precision(void);
 // A/B kernel-selection switches (focr_core.hip focr_set_tuning)

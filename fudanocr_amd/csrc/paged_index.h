@@ -1,0 +1,63 @@
+// Index arithmetic of the paged key / value cache, for the kernels of paged_attention.hip and beam.hip.  Plain C++ with no
+// device intrinsics, so that a host program can check every function over whole ranges.
+//
+// Layout: pages [num_pages][heads][page][dim]; row s of `table` names the pages of sequence s in order; kv_lens[s] tokens are
+// in the cache, the new ones included.  All three come from device memory and are not trusted: a sequence whose numbers do
+// not fit is `bad` (its results are NaN, nothing of it is written to the cache) and no address is formed from them.
+#pragma once
+#ifdef __HIPCC__
+#define PG_FN __host__ __device__ __forceinline__
+#else
+#define PG_FN static inline
+#endif
+
+struct PagedShape {
+  const int* table;    // [seqs][table_ld]
+  const int* kv_lens;  // [seqs]
+  const int* q_start;  // [seqs + 1] first row of each sequence's new tokens, or null: tokens / seqs rows each
+  long tokens, num_pages;
+  int seqs, table_ld, page_shift, max_kv;
+};
+
+struct PagedSeq {
+  long t0;   // first row of the new tokens
+  int n;     // how many
+  int len;   // tokens in the cache
+  bool bad;  // kv_lens[s] out of range
+};
+
+// rows of sequence s: an offset pair that does not lie in order inside [0, tokens] owns no rows
+PG_FN PagedSeq paged_seq(const PagedShape& c, int s) {
+  PagedSeq r;
+  if (c.q_start) {
+    const long a = c.q_start[s], b = c.q_start[s + 1];
+    const bool ok = a >= 0 && b >= a && b <= c.tokens;
+    r.t0 = ok ? a : 0;
+    r.n = ok ? (int)(b - a) : 0;
+  } else {
+    r.n = (int)(c.tokens / c.seqs);
+    r.t0 = (long)s * r.n;
+  }
+  const int len = c.kv_lens[s];
+  r.bad = len < 0 || len > c.max_kv || len > ((long)c.table_ld << c.page_shift);
+  r.len = r.bad ? 0 : len;
+  return r;
+}
+
+// page that holds position pos of sequence s, or -1 when the table names none
+PG_FN int paged_page(const PagedShape& c, int s, int pos) {
+  const int p = c.table[(long)s * c.table_ld + (pos >> c.page_shift)];
+  return p >= 0 && p < c.num_pages ? p : -1;
+}
+
+// keys that new token i of n sees: a prefix of the cache
+PG_FN int paged_visible(int len, int n, int i, int causal) {
+  const int v = causal ? len - n + 1 + i : len;
+  return v < 0 ? 0 : v;
+}
+
+// A flat list of row tiles over sequences of unknown lengths: `rows` rows per new token (the heads that share a key), `tile`
+// rows per tile.  Sequence s owns the tiles from first(s) on; first(s + 1) - first(s) >= ceil(n * rows / tile) for every
+// length, so first(seqs) tiles are enough, and first() is monotone: a tile finds its sequence by search.
+PG_FN long paged_first_tile(long t0, int s, int rows, int tile) { return t0 * rows / tile + s; }
+PG_FN long paged_tiles(long tokens, int seqs, int rows, int tile) { return tokens * rows / tile + seqs; }

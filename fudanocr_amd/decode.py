@@ -1,0 +1,267 @@
+"""Autoregressive decoding on the HIP kernels (csrc/paged_attention.hip, csrc/beam.hip): a paged key / value cache, attention
+of new tokens over it, beam search's selection and the reordering of the surviving beams' caches.
+
+The recognizers' `beam_search` (fudanocr_amd/sld/beam.py) is built from these; they work on their own as well.  Unlike the
+training operators of `kernels` / `sld.ops` they also take bf16 and fp16 tensors, keep no graph, and nothing in them waits
+for the device: lengths, tables and parents stay there.
+
+A cache is four tensors:
+
+* ``k_pages``, ``v_pages``  [num_pages, heads, page, dim]: `page` (a power of two from 8 to 1024) tokens a page;
+* ``table``    int32 [seqs, pages per sequence]: row s names the pages of sequence s in order;
+* ``kv_lens``  int32 [seqs]: tokens of each sequence in the cache, the new ones of the present call included.
+
+A chunk of new tokens is one packed tensor [tokens, heads, dim]: ``q_start`` (int32 [seqs + 1], non-decreasing) gives the first
+row of every sequence, without it each has tokens / seqs rows.  Rows of no sequence (in front of the first, behind the last)
+are left as they are.  The new tokens of a sequence are its last ones: the first of n has position kv_lens - n.
+
+What comes from the device is checked there: a length beyond the table or `max_kv`, or more new tokens than `max_q`, makes a
+sequence's output NaN, a page number outside the cache that of the tokens that need the page (other tokens of the sequence
+may be NaN then too); nothing outside the given tensors is read or written."""
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+from .kernels import _RAW_STREAM
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _need(ok, what):
+    if not ok:
+        raise RuntimeError("fudanocr_amd.decode: " + what)
+
+
+def _launch(device, name, *args):
+    """the entry point on the current stream of the tensors' device, whatever device is current"""
+    _need(device.type == "cuda", "tensors must be on the GPU, got %s" % device)
+    if device.index == torch.cuda.current_device():
+        _lib.call(name, *args, _stream(device))
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args, _stream(device))
+
+
+def _stream(device):
+    return _RAW_STREAM(device.index) if _RAW_STREAM is not None else torch.cuda.current_stream(device).cuda_stream
+
+
+def _int32(t, shape, device, what):
+    _need(isinstance(t, torch.Tensor) and t.dtype == torch.int32 and tuple(t.shape) == tuple(shape) and t.is_contiguous()
+          and t.device == device, "%s must be a contiguous int32 tensor %s on %s" % (what, list(shape), device))
+
+
+def _cache(k_pages, v_pages, table, kv_lens, q_start):
+    _need(k_pages.dim() == 4 and k_pages.shape == v_pages.shape and k_pages.dtype == v_pages.dtype
+          and k_pages.dtype in _DTYPES, "k_pages and v_pages must be two [num_pages, heads, page, dim] tensors of one type "
+          "(fp32, bf16 or fp16)")
+    _need(k_pages.is_contiguous() and v_pages.is_contiguous() and k_pages.device == v_pages.device,
+          "k_pages and v_pages must be contiguous and on one device")
+    num_pages, heads, page, dim = k_pages.shape
+    _need(8 <= page <= 1024 and page & (page - 1) == 0, "page must be a power of two from 8 to 1024, got %d" % page)
+    _need(dim in (64, 128, 256), "head dim must be 64, 128 or 256, got %d" % dim)
+    _need(num_pages > 0 and heads > 0, "the cache has no pages or no heads")
+    dev = k_pages.device
+    _need(isinstance(table, torch.Tensor) and table.dim() == 2 and table.shape[1] > 0, "table must be [seqs, pages per sequence]")
+    seqs = table.shape[0]
+    _int32(table, table.shape, dev, "table")
+    _int32(kv_lens, (seqs,), dev, "kv_lens")
+    if q_start is not None:
+        _int32(q_start, (seqs + 1,), dev, "q_start")
+    return num_pages, heads, page, dim, seqs
+
+
+def _rows(t, heads, dim, like, what):
+    _need(t.dim() == 3 and t.shape[2] == dim and (heads is None or t.shape[1] == heads) and t.dtype == like.dtype
+          and t.device == like.device, "%s must be [tokens, %s, %d] %s on %s"
+          % (what, "heads" if heads is None else heads, dim, like.dtype, like.device))
+    _need(t.stride(2) == 1 or t.numel() == 0, "%s must have contiguous rows of dim" % what)
+
+
+def _even(tokens, seqs, q_start):
+    _need(q_start is not None or seqs == 0 or tokens % seqs == 0,
+          "without q_start every sequence has the same number of rows; %d tokens, %d sequences" % (tokens, seqs))
+
+
+def paged_append(k_new, v_new, k_pages, v_pages, table, kv_lens, q_start=None):
+    """writes the new tokens' keys and values [tokens, heads, dim] to their pages (positions kv_lens - n .. kv_lens - 1 of each
+    sequence).  A token whose page the table does not name is dropped."""
+    num_pages, heads, page, dim, seqs = _cache(k_pages, v_pages, table, kv_lens, q_start)
+    _rows(k_new, heads, dim, k_pages, "k_new")
+    _rows(v_new, heads, dim, k_pages, "v_new")
+    tokens = k_new.shape[0]
+    _need(v_new.shape[0] == tokens, "k_new and v_new must have the same tokens")
+    _even(tokens, seqs, q_start)
+    if tokens == 0 or seqs == 0:
+        return
+    _launch(k_pages.device, "focr_paged_append", k_new.data_ptr(), v_new.data_ptr(), k_new.stride(0), k_new.stride(1),
+            v_new.stride(0), v_new.stride(1), k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), kv_lens.data_ptr(),
+            None if q_start is None else q_start.data_ptr(), tokens, seqs, heads, dim, page, table.shape[1], num_pages,
+            _DTYPES[k_pages.dtype])
+
+
+def paged_attention(q, k_pages, v_pages, table, kv_lens, q_start=None, causal=True, scale=None, max_q=None, max_kv=None,
+                    out=None):
+    """softmax(scale q k^T) v of the new tokens q [tokens, heads, dim] over their sequences' caches -> [tokens, heads, dim].
+
+    heads is a multiple of the cache's; head h reads the cache's head h // (heads / cache heads).  causal: a token at position p
+    sees the positions 0 .. p, else all kv_lens of them; a token that sees nothing gets zeros.  scale: 1 / sqrt(dim) unless
+    given, positive.  max_q / max_kv: bounds on a sequence's new tokens and on kv_lens that the caller knows (they size the
+    launch; the defaults are the most the tensors allow).  out: where to write (not q's memory)."""
+    num_pages, kv_heads, page, dim, seqs = _cache(k_pages, v_pages, table, kv_lens, q_start)
+    _rows(q, None, dim, k_pages, "q")
+    tokens, heads = q.shape[0], q.shape[1]
+    _need(heads > 0 and heads % kv_heads == 0, "%d heads over a cache of %d" % (heads, kv_heads))
+    _even(tokens, seqs, q_start)
+    scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
+    _need(0.0 < scale < math.inf, "scale must be positive and finite, got %r" % scale)
+    limit = table.shape[1] * page
+    max_kv = limit if max_kv is None else min(int(max_kv), limit)
+    if q_start is None:
+        max_q = tokens // seqs if seqs else 0
+    else:
+        max_q = tokens if max_q is None else min(int(max_q), tokens)
+    _need(max_q >= 0 and 0 <= max_kv < 2 ** 31, "max_q / max_kv out of range")
+    if out is None:
+        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
+    else:
+        _rows(out, heads, dim, k_pages, "out")
+        _need(out.shape[0] == tokens, "out must have q's shape")
+        _need(not _overlap(out, q), "out must not share q's memory")
+    if tokens == 0 or seqs == 0:
+        return out
+    dt, dev = _DTYPES[q.dtype], q.device
+    n_ws = _lib.load().focr_paged_attention_ws_bytes(tokens, seqs, heads, kv_heads, dim, max_q, max_kv, dt)
+    _need(n_ws >= 0, "arguments out of range")
+    ws = torch.empty(n_ws, dtype=torch.uint8, device=dev) if n_ws else None
+    _launch(dev, "focr_paged_attention_fwd", q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(), v_pages.data_ptr(),
+            table.data_ptr(), kv_lens.data_ptr(), None if q_start is None else q_start.data_ptr(), out.data_ptr(),
+            out.stride(0), out.stride(1), None if ws is None else ws.data_ptr(), n_ws, tokens, seqs, heads, kv_heads, dim, page,
+            table.shape[1], num_pages, max_q, max_kv, scale, int(bool(causal)), dt)
+    return out
+
+
+def _overlap(a, b):
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+def beam_select(logits, scores, finished=None, eos=None, n=None):
+    """the n (default: beams) best continuations of every batch entry over beams and vocabulary, best first.
+
+    logits [batch, beams, vocab] (fp32, bf16 or fp16; rows contiguous), scores fp32 [batch, beams]: the beams' running
+    log-probabilities (-inf: no such beam, as for all but the first at a search's first step).  A candidate's score is its beam's
+    plus the token's log-softmax; a finished beam (bool [batch, beams]) has the one candidate (itself, eos) at its own score.
+    Equal scores go to the lowest (beam, token).  NaN logits and beams whose score or normaliser is not finite rank as -inf.
+
+    -> (scores fp32 [batch, n], parents int32 [batch, n], tokens int64 [batch, n], finished bool [batch, n])"""
+    _need(logits.dim() == 3 and logits.dtype in _DTYPES, "logits must be [batch, beams, vocab] in fp32, bf16 or fp16")
+    batch, beams, vocab = logits.shape
+    dev = logits.device
+    n = beams if n is None else int(n)
+    _need(1 <= beams <= 64 and 1 <= n <= 64 and vocab >= 1 and n <= beams * vocab,
+          "beams and n must be 1 to 64 and n at most beams * vocab; got %d beams, n = %d, vocab %d" % (beams, n, vocab))
+    _need(logits.stride(2) == 1 or vocab == 1 or logits.numel() == 0, "logits must have contiguous rows of vocab")
+    _need(scores.dtype == torch.float32 and tuple(scores.shape) == (batch, beams) and scores.is_contiguous()
+          and scores.device == dev, "scores must be a contiguous fp32 tensor %s on %s" % ([batch, beams], dev))
+    if finished is not None:
+        _need(finished.dtype == torch.bool and tuple(finished.shape) == (batch, beams) and finished.is_contiguous()
+              and finished.device == dev, "finished must be a contiguous bool tensor %s on %s" % ([batch, beams], dev))
+        _need(eos is not None, "finished beams need an eos")
+    _need(eos is None or 0 <= int(eos) < vocab, "eos must be inside the vocabulary")
+    eos = -1 if eos is None else int(eos)
+    out = (torch.empty((batch, n), dtype=torch.float32, device=dev), torch.empty((batch, n), dtype=torch.int32, device=dev),
+           torch.empty((batch, n), dtype=torch.int64, device=dev), torch.empty((batch, n), dtype=torch.bool, device=dev))
+    if batch == 0:
+        return out
+    dt = _DTYPES[logits.dtype]
+    n_ws = _lib.load().focr_beam_select_ws_bytes(batch, beams, vocab, n, dt)
+    ws = torch.empty(n_ws, dtype=torch.uint8, device=dev) if n_ws else None
+    _launch(dev, "focr_beam_select", logits.data_ptr(), logits.stride(0), logits.stride(1), scores.data_ptr(),
+            None if finished is None else finished.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(),
+            out[3].data_ptr(), None if ws is None else ws.data_ptr(), n_ws, batch, beams, vocab, n, eos, dt)
+    return out
+
+
+def beam_reorder(parents, table, kv_lens, spare, pages, table_out=None, spare_out=None):
+    """beam j of every group goes on from its group's beam parents[group, j]: -> (table, spare) of the reordered beams.
+
+    parents int32 [groups, beams]; the cache's sequences are the groups' beams in order, and the beams of a group have the same
+    kv_lens (the first one's counts).  Full pages are shared by table entry; the partial last page is copied to the beam's page
+    in `spare` (int32 [seqs]), and the one it had becomes its spare.  pages: the page tensors (k_pages and v_pages of every
+    layer) that the table stands for.  Before the call, the pages in `spare` and each beam's entries from its partial page on
+    must be its own alone (`PagedCache` sees to that).  table_out / spare_out may be the inputs; a parent outside
+    the group counts as the beam itself."""
+    _need(isinstance(parents, torch.Tensor) and parents.dim() == 2, "parents must be [groups, beams]")
+    groups, beams = parents.shape
+    dev, slots = parents.device, groups * beams
+    _int32(parents, parents.shape, dev, "parents")
+    _need(1 <= beams <= 64 and slots <= 65535, "beams must be 1 to 64 and groups * beams at most 65535")
+    _need(table.dim() == 2 and table.shape[0] == slots and table.shape[1] > 0, "table must be [groups * beams, pages per sequence]")
+    _int32(table, table.shape, dev, "table")
+    _int32(kv_lens, (slots,), dev, "kv_lens")
+    _int32(spare, (slots,), dev, "spare")
+    pages = list(pages)
+    _need(len(pages) > 0, "no page tensors")
+    for p in pages:
+        _need(p.dim() == 4 and p.shape == pages[0].shape and p.dtype == pages[0].dtype and p.dtype in _DTYPES
+              and p.is_contiguous() and p.device == dev, "pages must be contiguous [num_pages, heads, page, dim] tensors of one "
+              "shape and type (fp32, bf16 or fp16) on %s" % dev)
+    num_pages, heads, page, dim = pages[0].shape
+    _need(8 <= page <= 1024 and page & (page - 1) == 0, "page must be a power of two from 8 to 1024, got %d" % page)
+    _need(num_pages > 0 and heads > 0 and dim > 0 and dim * pages[0].element_size() % 16 == 0,
+          "rows of dim must be whole 16-byte units")
+    table_out = torch.empty_like(table) if table_out is None else table_out
+    spare_out = torch.empty_like(spare) if spare_out is None else spare_out
+    _int32(table_out, table.shape, dev, "table_out")
+    _int32(spare_out, spare.shape, dev, "spare_out")
+    if slots:
+        ptrs = (ctypes.c_void_p * len(pages))(*[p.data_ptr() for p in pages])
+        _launch(dev, "focr_beam_reorder", parents.data_ptr(), table.data_ptr(), kv_lens.data_ptr(), spare.data_ptr(),
+                table_out.data_ptr(), spare_out.data_ptr(), ptrs, len(pages), groups, beams, heads, dim, page, table.shape[1],
+                num_pages, _DTYPES[pages[0].dtype])
+    return table_out, spare_out
+
+
+class PagedCache:
+    """The caches of a decoder's layers for `seqs` sequences of at most max_len tokens: page tensors per layer, one table, the
+    lengths and a spare page per sequence.  Every sequence starts with pages of its own.
+
+    step (n new tokens for every sequence):  cache.advance(n);  per layer: cache.append(layer, k, v), cache.attend(layer, q);
+    between the steps of a beam search: cache.reorder(parents)."""
+
+    def __init__(self, seqs, max_len, heads, dim, layers=1, page=16, dtype=torch.float32, device="cuda"):
+        _need(seqs > 0 and max_len > 0 and heads > 0 and layers > 0, "seqs, max_len, heads and layers must be positive")
+        _need(8 <= page <= 1024 and page & (page - 1) == 0, "page must be a power of two from 8 to 1024, got %d" % page)
+        _need(dim in (64, 128, 256) and dtype in _DTYPES, "head dim must be 64, 128 or 256, the type fp32, bf16 or fp16")
+        per = -(-max_len // page)
+        num = seqs * (per + 1)
+        _need(num < 2 ** 31, "more pages than int32 numbers")
+        self.page, self.max_len, self.length = page, max_len, 0
+        self.k = [torch.empty((num, heads, page, dim), dtype=dtype, device=device) for _ in range(layers)]
+        self.v = [torch.empty((num, heads, page, dim), dtype=dtype, device=device) for _ in range(layers)]
+        ids = torch.arange(num, dtype=torch.int32, device=device)
+        self.table, self.spare = ids[:seqs * per].view(seqs, per), ids[seqs * per:].clone()
+        self.kv_lens = torch.zeros(seqs, dtype=torch.int32, device=device)
+
+    def advance(self, n):
+        """n more tokens for every sequence (their keys and values follow with `append`)"""
+        _need(n >= 0 and self.length + n <= self.max_len, "%d + %d tokens in a cache of %d" % (self.length, n, self.max_len))
+        self.length += n
+        self.kv_lens += n
+
+    def append(self, layer, k_new, v_new):
+        paged_append(k_new, v_new, self.k[layer], self.v[layer], self.table, self.kv_lens)
+
+    def attend(self, layer, q, causal=True, scale=None, out=None):
+        return paged_attention(q, self.k[layer], self.v[layer], self.table, self.kv_lens, causal=causal, scale=scale,
+                               max_kv=self.length, out=out)
+
+    def reorder(self, parents):
+        beam_reorder(parents, self.table, self.kv_lens, self.spare, self.k + self.v, self.table, self.spare)

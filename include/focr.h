@@ -475,6 +475,38 @@ int focr_weight_cross_entropy_masked_fwd(const float* logits, const long long* t
                                          float* nll_ws, float* grad, long rows, int C, const long long* plan,
                                          focr_stream_t stream);
 
+/* ---- autoregressive decoding of the transformer recognizers: paged key / value cache, attention of new tokens over it,
+ * beam search (csrc/paged_attention.hip, csrc/beam.hip; Python: fudanocr_amd/decode.py, which states the layouts in full).
+ * dtype: 0 fp32, 1 bf16, 2 fp16 -- of q, o, the new keys / values, the pages and the logits; ld* = strides in elements of the
+ * token and head axes (rows of dim contiguous).  Pages [num_pages][heads][page][dim], page a power of two 8..1024, dim 64 / 128 /
+ * 256; table [seqs][table_ld], kv_lens [seqs] (new tokens included), q_start [seqs + 1] or NULL (tokens / seqs rows each): all
+ * int32 in device memory and checked by the kernels -- a sequence whose numbers do not fit gets NaN, nothing outside the given
+ * buffers is read or written. */
+#define FOCR_DT_F32 0
+#define FOCR_DT_BF16 1
+#define FOCR_DT_F16 2
+int focr_paged_append(const void* k_new, const void* v_new, long ldtk, long ldhk, long ldtv, long ldhv, void* k_pages,
+                      void* v_pages, const int* table, const int* kv_lens, const int* q_start, long tokens, int seqs, int heads,
+                      int dim, int page, int table_ld, long num_pages, int dtype, focr_stream_t stream);
+/* ws: focr_paged_attention_ws_bytes() bytes (0: may be NULL; negative: arguments out of range); max_q / max_kv bound a
+ * sequence's new tokens and kv_lens (they size the launch; a sequence beyond them gets NaN) */
+long focr_paged_attention_ws_bytes(long tokens, int seqs, int heads, int kv_heads, int dim, int max_q, int max_kv, int dtype);
+int focr_paged_attention_fwd(const void* q, long ldt, long ldh, const void* k_pages, const void* v_pages, const int* table,
+                             const int* kv_lens, const int* q_start, void* o, long ldto, long ldho, void* ws, long ws_bytes,
+                             long tokens, int seqs, int heads, int kv_heads, int dim, int page, int table_ld, long num_pages,
+                             int max_q, int max_kv, float scale, int causal, int dtype, focr_stream_t stream);
+/* logits [batch][beams][vocab] (ldb / ldk: strides of the first two axes), scores fp32 [batch][beams], finished uint8 (may be
+ * NULL); the n best candidates score + log_softmax, ties to the lowest (beam, token); ws: focr_beam_select_ws_bytes() */
+long focr_beam_select_ws_bytes(int batch, int beams, int vocab, int n, int dtype);
+int focr_beam_select(const void* logits, long ldb, long ldk, const float* scores, const uint8_t* finished, float* out_scores,
+                     int* out_parents, long long* out_tokens, uint8_t* out_finished, void* ws, long ws_bytes, int batch,
+                     int beams, int vocab, int n, int eos, int dtype, focr_stream_t stream);
+/* parents [groups][beams]; slots = groups * beams rows of table / kv_lens / spare; pages: HOST array of `tensors` device
+ * pointers to page tensors of one shape; table_out / spare_out may be table / spare */
+int focr_beam_reorder(const int* parents, const int* table, const int* kv_lens, const int* spare, int* table_out,
+                      int* spare_out, void* const* pages, int tensors, int groups, int beams, int heads, int dim, int page,
+                      int table_ld, long num_pages, int dtype, focr_stream_t stream);
+
 /* ---- data-parallel gradient exchange (RCCL over xGMI; replaces nn.DataParallel's gather of the gradients,
  * reference interfaces/base.py:178-179).  One communicator per process = per GPU.  RCCL is bound at run time.
  * focr_comm_unique_id: rank 0 draws the 128-byte id (sizeof(ncclUniqueId)) and gives it to every rank by a host channel;
