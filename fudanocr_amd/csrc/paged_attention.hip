@@ -114,6 +114,485 @@ __global__ __launch_bounds__(256) void paged_attention_row_kernel(const T* __res
     o[t * ldto + h * ldho + e * 64 + lane] = (T)(bad ? NAN : l == 0.f ? 0.f : acc[e] / l);
 }
 
+// ---- matrix instructions -----------------------------------------------------------------------------------------------
+// Operands are 16-byte chunks of a row: 8 16-bit or 4 fp32 values of the contraction axis.  Lane l of a 16 x 16 tile holds row
+// l % 16 of A (column l % 16 of B) at chunk l / 16, lane l of the 32 x 32 tile row l % 32 at chunk l / 32; any order of the
+// contraction axis will do as long as A and B share it.  Results: column l % 16, rows 4 (l / 16) + i, or column l % 32, rows
+// 8 (i / 4) + 4 (l / 32) + i % 4.  fp32 runs on the exact fp32 instructions, one value of the chunk at a time.
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+template <typename T> struct PgMma;
+template <> struct PgMma<bf16_t> {
+  static __device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(focr_bf16x8, a), __builtin_bit_cast(focr_bf16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(focr_bf16x8, a), __builtin_bit_cast(focr_bf16x8, b), c, 0, 0, 0);
+  }
+  static constexpr uint32_t EXP = 0x7f80u, ONE = 0x3f80u;
+};
+template <> struct PgMma<f16_t> {
+  static __device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  static constexpr uint32_t EXP = 0x7c00u, ONE = 0x3c00u;
+};
+template <> struct PgMma<float> {
+  static __device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[i]), __uint_as_float(b[i]), c, 0, 0, 0);
+    return c;
+  }
+  static __device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[i]), __uint_as_float(b[i]), c, 0, 0, 0);
+    return c;
+  }
+  static constexpr uint32_t EXP = 0x7f800000u, ONE = 0x3f800000u;
+};
+
+// two fp32 values as a 16-bit pair, rounded to nearest: the weights p lie in [0, 1] relative to the running maximum, so a
+// weight loses at most half a step of the output's own type and the errors of a row's keys average out
+template <typename T> __device__ __forceinline__ uint32_t pg_pack(float a, float b);
+template <> __device__ __forceinline__ uint32_t pg_pack<bf16_t>(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, focr_bf16x2));
+}
+template <> __device__ __forceinline__ uint32_t pg_pack<f16_t>(float a, float b) {
+  typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
+}
+
+// a word of values with its infinities and NaN replaced by zero
+template <typename T> __device__ __forceinline__ uint32_t pg_finite(uint32_t w) {
+  if constexpr (sizeof(T) == 4) return (w & 0x7f800000u) == 0x7f800000u ? 0u : w;
+  const uint32_t e = PgMma<T>::EXP;
+  if ((w & e) == e) w &= 0xffff0000u;
+  if ((w >> 16 & e) == e) w &= 0xffffu;
+  return w;
+}
+// one where a chunk holds +inf (CLS 1), -inf (2) or NaN (3), zero elsewhere
+template <typename T, int CLS> __device__ __forceinline__ u32x4 pg_class(u32x4 a) {
+  u32x4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      const uint32_t w = a[i];
+      r[i] = (CLS == 1 ? w == 0x7f800000u : CLS == 2 ? w == 0xff800000u : (w & 0x7fffffffu) > 0x7f800000u) ? 0x3f800000u : 0u;
+    } else {
+      uint32_t out = 0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t w = a[i] >> (16 * h) & 0xffffu, e = PgMma<T>::EXP;
+        const bool hit = CLS == 1 ? w == e : CLS == 2 ? w == (e | 0x8000u) : (w & 0x7fffu) > e;
+        out |= (hit ? PgMma<T>::ONE : 0u) << (16 * h);
+      }
+      r[i] = out;
+    }
+  }
+  return r;
+}
+// what a sum of p v becomes when it also holds `pos` values +inf, `neg` values -inf and `nan` NaN
+__device__ __forceinline__ float pg_with_nonfinite(float x, float pos, float neg, float nan) {
+  if (pos > 0.f) x += INFINITY;
+  if (neg > 0.f) x -= INFINITY;
+  return nan > 0.f ? NAN : x;
+}
+
+// a part's sum of weights relative to the common maximum; a part without keys has sum 0 at maximum -inf, one whose scores are
+// all NaN has a NaN sum there, which must not get lost
+__device__ __forceinline__ float pg_share(float sum, float log2_ratio) {
+  return sum == 0.f ? 0.f : sum != sum ? sum : sum * __builtin_amdgcn_exp2f(log2_ratio);
+}
+
+template <typename T>
+struct PgArgs {
+  const T* q;
+  long ldt, ldh;
+  const T *kp, *vp;
+  PagedShape c;
+  T* o;
+  long ldto, ldho;
+  float* part;   // [split][token][head][D], weights relative to the split's own maximum
+  float2* ml;    // [split][token][head]: that maximum (in log2 units) and the sum of the weights
+  int max_q, heads, kv_heads, group, nsplit, chunk, causal, thin_rows, wide_q, wide_o;
+  float c2;      // scale * log2(e)
+};
+
+template <typename T, int N> __device__ __forceinline__ void pg_store_row(T* p, const float (&v)[N], bool wide) {
+  if (wide) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < N; i += 4) *(f32x4*)(p + i) = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
+    } else {
+      uint32_t w[N / 2];
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) w[i] = pg_pack<T>(v[2 * i], v[2 * i + 1]);
+      if constexpr (N == 8) *(u32x4*)p = u32x4{w[0], w[1], w[2], w[3]};
+      else *(uint2*)p = uint2{w[0], w[1]};
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = (T)v[i];
+  }
+}
+
+// 16-byte chunk of a query row
+template <typename T> __device__ __forceinline__ u32x4 pg_load_chunk(const T* p, bool wide) {
+  if (wide) return *(const u32x4*)p;
+  if constexpr (sizeof(T) == 4) {
+    return u32x4{__float_as_uint(p[0]), __float_as_uint(p[1]), __float_as_uint(p[2]), __float_as_uint(p[3])};
+  } else {
+    const uint16_t* w = (const uint16_t*)p;
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = w[2 * i] | (uint32_t)w[2 * i + 1] << 16;
+    return r;
+  }
+}
+
+// rows of a sequence whose numbers do not fit: NaN
+template <typename T, int D>
+__device__ __forceinline__ void pg_fill_nan(const PgArgs<T>& a, const PagedSeq& sq, int kh, int threads) {
+  const long total = (long)sq.n * a.group * D;
+  for (long i = threadIdx.x; i < total; i += threads) {
+    const long r = i / D;
+    a.o[(sq.t0 + r / a.group) * a.ldto + (kh * a.group + r % a.group) * a.ldho + i % D] = (T)NAN;
+  }
+}
+
+// ======================================================================================================================
+// Few rows (one token, or a few tokens and the heads that share a key head: up to 16 NT rows), a long axis of keys: bound by
+// the bytes of the keys and values, which are read once, straight into registers in the matrix instructions' own layout -- no
+// LDS, no barrier in the loop, 4 waves a block that take every fourth tile of KT keys and are joined at the end.
+//   S^T = K Q^T   A = 16 keys x chunk (lane: key l % 16, chunk l / 16 + 4 u), B = queries from registers;
+//   O^T = V^T P^T  the lane that holds column q of S^T holds the weights of keys 4 (l / 16) + i: already B's layout when the
+//                 contraction index means those keys.  A = V^T needs, per lane, these keys' values at ONE d: the lane loads the
+//                 NK keys' rows at d = CH (l % 16) .. + CH (16 lanes = whole row, coalesced) and transposes its NK x CH square in
+//                 registers (v_perm, 16-bit types; a choice of registers in fp32); tile (u, c) of O^T then has row e <-> d =
+//                 16 CH u + CH e + c.
+// The next tile's loads go out between the two products.  MFMA time is a tenth of the bytes' (16-bit) to a third (fp32).
+// ======================================================================================================================
+#define PG_MAX_CHUNK 8192
+template <typename T, int D, int NT> constexpr int pg_thin_waves() { return D * NT <= 0 ? 4 : 1; }
+template <typename T, int D, int NT>
+__global__ __launch_bounds__(256, (pg_thin_waves<T, D, NT>())) void paged_thin_kernel(PgArgs<T> a) {
+  constexpr int ES = sizeof(T), EC = 16 / ES;          // elements of a chunk
+  constexpr int NU = D * ES / 64;                      // chunk quads of a row (S^T contraction steps)
+  constexpr int NK = ES == 4 ? 4 : 8, KT = 4 * NK;     // keys of a lane, keys of a tile
+  constexpr int CH = (D / 16 < EC) ? D / 16 : EC, VU = D / (16 * CH);  // values of one V load, loads per row
+  constexpr int PITCH = D + 4;
+  __shared__ int pages[PG_MAX_CHUNK / 8 + 2];
+  __shared__ float red[16 * NT * PITCH];
+  __shared__ float2 wml[4][16 * NT];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, g = lane >> 4;
+  const int split = blockIdx.x % a.nsplit;
+  const int kh = blockIdx.x / a.nsplit % a.kv_heads, s = blockIdx.x / a.nsplit / a.kv_heads;
+  const PagedShape& c = a.c;
+  const PagedSeq sq = paged_seq(c, s);
+  if ((long)sq.n * a.group > a.thin_rows && sq.n <= a.max_q) return;     // the other kernel's
+  if (sq.n == 0) return;
+  if (sq.bad || sq.n > a.max_q) {
+    if (split == 0 && (sq.n <= a.max_q || a.thin_rows >= a.max_q * a.group)) pg_fill_nan<T, D>(a, sq, kh, 256);
+    return;
+  }
+  const int R = sq.n * a.group;
+  const int vmin = paged_visible(sq.len, sq.n, 0, a.causal), kend = paged_visible(sq.len, sq.n, sq.n - 1, a.causal);
+  const int k0 = split * a.chunk;
+  const bool direct = sq.len <= a.chunk;
+  if (split && k0 >= kend) return;
+  const int k1 = kend < k0 + a.chunk ? kend : k0 + a.chunk;
+
+  // page numbers of this block's keys; one that names no page makes every row NaN
+  int any_bad = 0;
+  const int p0 = k0 >> c.page_shift, np = k1 > k0 ? ((k1 - 1) >> c.page_shift) - p0 + 1 : 0;
+  for (int i = tid; i < np; i += 256) {
+    const int p = paged_page(c, s, (p0 + i) << c.page_shift);
+    any_bad |= p < 0;
+    pages[i] = p < 0 ? 0 : p;
+  }
+  any_bad = __syncthreads_or(any_bad);
+
+  u32x4 qf[NT][NU];
+  int vis[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int r = t * 16 + l16;
+    const bool ok = r < R;
+    const int i = ok ? r / a.group : 0, h = kh * a.group + (ok ? r - i * a.group : 0);
+    vis[t] = ok ? paged_visible(sq.len, sq.n, i, a.causal) : 0;
+    const T* p = a.q + (sq.t0 + i) * a.ldt + h * a.ldh + g * EC;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) qf[t][u] = ok ? pg_load_chunk(p + u * 4 * EC, a.wide_q) : u32x4{0, 0, 0, 0};
+  }
+
+  const long head_bytes = ((long)D * ES) << c.page_shift, page_bytes = head_bytes * a.kv_heads;
+  const char *kbase = (const char*)a.kp + kh * head_bytes, *vbase = (const char*)a.vp + kh * head_bytes;
+  const int slot_mask = (1 << c.page_shift) - 1;
+  u32x4 kr[KT / 16][NU];
+  uint32_t vr[NK][VU * CH * ES / 4];
+  auto row_at = [&](int key) { return pages[(key >> c.page_shift) - p0] * page_bytes + (long)(key & slot_mask) * (D * ES); };
+  auto load_k = [&](int base) {
+#pragma unroll
+    for (int sub = 0; sub < KT / 16; ++sub) {
+      const int key = base + sub * 16 + l16;
+      const char* p = kbase + row_at(key < k1 ? key : k1 - 1) + g * 16;
+#pragma unroll
+      for (int u = 0; u < NU; ++u) kr[sub][u] = *(const u32x4*)(p + u * 64);
+    }
+  };
+  auto load_v = [&](int base) {
+#pragma unroll
+    for (int qd = 0; qd < NK / 4; ++qd) {
+      // four keys that lie in one page; behind the last key: the quad that holds it (its tail may never have been written)
+      const int key = base + qd * 16 + 4 * g, last = (k1 - 1) & ~3;
+      const char* p = vbase + row_at(key < last ? key : last) + l16 * (CH * ES);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int u = 0; u < VU; ++u) {
+          const char* w = p + j * (D * ES) + u * (16 * CH * ES);
+          if constexpr (CH * ES == 16) {
+            const u32x4 x = *(const u32x4*)w;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) vr[qd * 4 + j][u * 4 + e] = x[e];
+          } else {
+            const uint2 x = *(const uint2*)w;
+            vr[qd * 4 + j][u * 2] = x.x;
+            vr[qd * 4 + j][u * 2 + 1] = x.y;
+          }
+        }
+    }
+  };
+  // A operand of O^T's tile (u, cc): this lane's keys at d = 16 CH u + CH (l % 16) + cc
+  auto v_frag = [&](int u, int cc) {
+    u32x4 r;
+    if constexpr (ES == 4) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r[j] = vr[j][u * CH + cc];
+    } else {
+      const int w = (u * CH + cc) / 2;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        r[j] = __builtin_amdgcn_perm(vr[2 * j + 1][w], vr[2 * j][w], (cc & 1) ? 0x07060302u : 0x05040100u);
+    }
+    return r;
+  };
+
+  f32x4 acc[NT][VU][CH];
+  float m[NT], l[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    m[t] = -INFINITY;
+    l[t] = 0.f;
+#pragma unroll
+    for (int u = 0; u < VU; ++u)
+#pragma unroll
+      for (int e = 0; e < CH; ++e) acc[t][u][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  int base = k0 + wave * KT;
+  if (base < k1) {
+    load_k(base);
+    load_v(base);
+  }
+  for (; base < k1; base += 4 * KT) {
+    const int next = base + 4 * KT;
+    f32x4 sc[NT][KT / 16];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int sub = 0; sub < KT / 16; ++sub) {
+        sc[t][sub] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < NU; ++u) sc[t][sub] = PgMma<T>::mma16(kr[sub][u], qf[t][u], sc[t][sub]);
+      }
+    if (next < k1) load_k(next);
+    if (base + KT > vmin) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int sub = 0; sub < KT / 16; ++sub)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (base + sub * 16 + 4 * g + i >= vis[t]) sc[t][sub][i] = -INFINITY;
+    }
+    u32x4 pf[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float mx = m[t];
+#pragma unroll
+      for (int sub = 0; sub < KT / 16; ++sub)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[t][sub][i]);
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float ref = mx == -INFINITY ? 0.f : mx * a.c2;
+      if (__any(mx > m[t])) {
+        const float al = __builtin_amdgcn_exp2f(m[t] * a.c2 - ref);
+        l[t] *= al;
+#pragma unroll
+        for (int u = 0; u < VU; ++u)
+#pragma unroll
+          for (int e = 0; e < CH; ++e) acc[t][u][e] *= al;
+        m[t] = mx;
+      }
+      float p[KT / 4];
+#pragma unroll
+      for (int sub = 0; sub < KT / 16; ++sub)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          p[sub * 4 + i] = __builtin_amdgcn_exp2f(fmaf(sc[t][sub][i], a.c2, -ref));
+          l[t] += p[sub * 4 + i];
+        }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (ES == 4) pf[t][j] = __float_as_uint(p[j]);
+        else pf[t][j] = pg_pack<T>(p[2 * j], p[2 * j + 1]);
+      }
+    }
+    if (base + KT > k1) {                              // behind the last key: whatever the page holds must not count
+#pragma unroll
+      for (int j = 0; j < NK; ++j)
+        if (base + (j / 4) * 16 + 4 * g + (j & 3) >= k1) {
+#pragma unroll
+          for (int w = 0; w < VU * CH * ES / 4; ++w) vr[j][w] = 0;
+        }
+    }
+    bool odd = false;                                  // 0 * inf: values that some of the rows do not see
+    if (base + KT > vmin && vmin < kend) {
+#pragma unroll
+      for (int j = 0; j < NK; ++j)
+#pragma unroll
+        for (int w = 0; w < VU * CH * ES / 4; ++w) odd |= pg_finite<T>(vr[j][w]) != vr[j][w];
+      odd = __any(odd);
+    }
+    if (odd) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        u32x4 see;                                     // one where this lane's key is visible to its row
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (ES == 4) see[j] = base + 4 * g + j < vis[t] ? 0x3f800000u : 0u;
+          else {
+            const int key = base + (j / 2) * 16 + 4 * g + (2 * j & 3);
+            see[j] = (key < vis[t] ? PgMma<T>::ONE : 0u) | (key + 1 < vis[t] ? PgMma<T>::ONE << 16 : 0u);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < VU; ++u)
+#pragma unroll
+          for (int e = 0; e < CH; ++e) {
+            const u32x4 vf = v_frag(u, e);
+            const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+            const f32x4 pos = PgMma<T>::mma16(pg_class<T, 1>(vf), see, z), neg = PgMma<T>::mma16(pg_class<T, 2>(vf), see, z);
+            const f32x4 nan = PgMma<T>::mma16(pg_class<T, 3>(vf), see, z);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[t][u][e][i] = pg_with_nonfinite(acc[t][u][e][i], pos[i], neg[i], nan[i]);
+            __builtin_amdgcn_sched_barrier(0);         // one tile at a time: this path must not cost the others registers
+          }
+      }
+#pragma unroll
+      for (int j = 0; j < NK; ++j)
+#pragma unroll
+        for (int w = 0; w < VU * CH * ES / 4; ++w) vr[j][w] = pg_finite<T>(vr[j][w]);
+    }
+#pragma unroll
+    for (int u = 0; u < VU; ++u)
+#pragma unroll
+      for (int e = 0; e < CH; ++e) {
+        const u32x4 vf = v_frag(u, e);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[t][u][e] = PgMma<T>::mma16(vf, pf[t], acc[t][u][e]);
+      }
+    if (next < k1) load_v(next);
+  }
+
+  // join the waves: one common maximum, then the sums one wave after the other (a fixed order)
+  const int nw = k1 - k0 > 3 * KT ? 4 : k1 - k0 > 2 * KT ? 3 : k1 - k0 > KT ? 2 : 1;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    l[t] += __shfl_xor(l[t], 16, 64);
+    l[t] += __shfl_xor(l[t], 32, 64);
+    if (g == 0) wml[wave][t * 16 + l16] = float2{m[t], l[t]};
+  }
+  __syncthreads();
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    float mx = wml[0][t * 16 + l16].x;
+    for (int w = 1; w < nw; ++w) mx = fmaxf(mx, wml[w][t * 16 + l16].x);
+    const float al = m[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[t] - mx) * a.c2);
+    for (int w = 0; w < nw; ++w) {
+      if (w == wave) {
+#pragma unroll
+        for (int u = 0; u < VU; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            f32x4* p = (f32x4*)&red[(t * 16 + l16) * PITCH + u * 16 * CH + (4 * g + i) * CH];
+#pragma unroll
+            for (int e = 0; e < CH; e += 4) {
+              f32x4 v = {acc[t][u][e][i] * al, acc[t][u][e + 1][i] * al, acc[t][u][e + 2][i] * al, acc[t][u][e + 3][i] * al};
+              if (w) v += p[e / 4];
+              p[e / 4] = v;
+            }
+          }
+      }
+      __syncthreads();
+    }
+  }
+  constexpr int N = ES == 4 ? 4 : 8;
+  for (int x = tid; x < R * (D / N); x += 256) {
+    const int r = x / (D / N), d = (x - r * (D / N)) * N, i = r / a.group, h = kh * a.group + r - i * a.group;
+    float mx = wml[0][r].x, ls = 0.f;
+    for (int w = 1; w < nw; ++w) mx = fmaxf(mx, wml[w][r].x);
+    for (int w = 0; w < nw; ++w) ls += pg_share(wml[w][r].y, (wml[w][r].x - mx) * a.c2);
+    if (any_bad) ls = NAN;
+    float v[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = red[r * PITCH + d + e];
+    if (direct) {
+      const float inv = ls == 0.f ? 0.f : 1.f / ls;
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[e] = ls == 0.f ? 0.f : v[e] * inv;
+      pg_store_row<T, N>(a.o + (sq.t0 + i) * a.ldto + h * a.ldho + d, v, a.wide_o);
+    } else {
+      const long row = ((long)split * c.tokens + sq.t0 + i) * a.heads + h;
+#pragma unroll
+      for (int e = 0; e < N; e += 4) *(f32x4*)(a.part + row * D + d + e) = f32x4{v[e], v[e + 1], v[e + 2], v[e + 3]};
+      if (d == 0) a.ml[row] = float2{any_bad ? 0.f : mx * a.c2, ls};
+    }
+  }
+}
+
+// ---- joins the splits of a row: one wave per (token, head) --------------------------------------------------------------
+template <typename T, int D>
+__global__ __launch_bounds__(256) void paged_join_kernel(PgArgs<T> a) {
+  constexpr int E = D / 64;
+  const int lane = threadIdx.x & 63;
+  const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= a.c.tokens * a.heads) return;
+  const long t = row / a.heads;
+  const int h = (int)(row - t * a.heads), s = pg_seq_of_row(a.c, t, lane);
+  const PagedSeq sq = paged_seq(a.c, s);
+  const long i = t - sq.t0;
+  if (i < 0 || i >= sq.n || sq.bad || sq.n > a.max_q || sq.len <= a.chunk) return;
+  const int n = (paged_visible(sq.len, sq.n, (int)i, a.causal) + a.chunk - 1) / a.chunk;
+  const long step = a.c.tokens * a.heads;
+  float mx = -INFINITY, ls = 0.f, v[E];
+  for (int e = 0; e < E; ++e) v[e] = 0.f;
+  for (int k = 0; k < n; ++k) mx = fmaxf(mx, a.ml[row + k * step].x);
+  for (int k = 0; k < n; ++k) {
+    const float2 ml = a.ml[row + k * step];
+    const float w = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mx);
+    ls += pg_share(ml.y, ml.x - mx);
+    const float* p = a.part + (row + k * step) * D + lane * E;
+    for (int e = 0; e < E; ++e) v[e] += w * p[e];
+  }
+  T* o = a.o + t * a.ldto + h * a.ldho + lane * E;
+  for (int e = 0; e < E; ++e) o[e] = (T)(ls == 0.f ? 0.f : v[e] / ls);
+}
+
 // ---- C entries ---------------------------------------------------------------------------------------------------------
 static bool pg_shape(PagedShape& c, const int* table, const int* kv_lens, const int* q_start, long tokens, int seqs, int page,
                      int table_ld, long num_pages, int max_kv) {
@@ -152,9 +631,60 @@ extern "C" int focr_paged_append(const void* k_new, const void* v_new, long ldtk
   return FOCR_OK;
 }
 
+// Splits of the key axis.  The keys of a (sequence, key head) go to blocks of `chunk` keys each, enough of them to fill the 256
+// CUs several times over even when most sequences are far shorter than the bound max_kv; a sequence of at most `chunk` keys
+// writes its output directly, the parts of a longer one are joined by a second launch.
+struct PgPlan {
+  int nsplit, chunk;
+};
+#ifndef PG_TARGET
+#define PG_TARGET 2048
+#endif
+#ifndef PG_MINCHUNK
+#define PG_MINCHUNK 256
+#endif
+static PgPlan pg_plan(int seqs, int kv_heads, int max_kv) {
+  const long groups = (long)seqs * kv_heads;
+  const long want = groups >= PG_TARGET ? 1 : (PG_TARGET + groups - 1) / groups;
+  long chunk = (max_kv + want - 1) / want;
+  chunk = (chunk + 127) / 128 * 128;
+  if (chunk < PG_MINCHUNK) chunk = PG_MINCHUNK;
+  if (chunk > PG_MAX_CHUNK) chunk = PG_MAX_CHUNK;
+  const int n = (int)((max_kv + chunk - 1) / chunk);
+  return {n > 0 ? n : 1, (int)chunk};
+}
+
 extern "C" long focr_paged_attention_ws_bytes(long tokens, int seqs, int heads, int kv_heads, int dim, int max_q, int max_kv,
                                               int dtype) {
-  return 0;
+  if (tokens <= 0 || seqs <= 0 || heads <= 0 || kv_heads <= 0 || dim <= 0 || max_q < 0 || max_kv < 0) return tokens == 0 || seqs == 0 ? 0 : -1;
+  const PgPlan p = pg_plan(seqs, kv_heads, max_kv);
+  return p.nsplit == 1 ? 0 : p.nsplit * tokens * heads * (dim + 2) * 4;
+}
+
+template <typename T, int D>
+static int pg_run(PgArgs<T> a, long ws_bytes, int dim, hipStream_t st) {
+  const PagedShape& c = a.c;
+  const PgPlan p = pg_plan(c.seqs, a.kv_heads, c.max_kv);
+  a.nsplit = p.nsplit;
+  a.chunk = p.chunk;
+  const long rows = c.tokens * a.heads;
+  if (p.nsplit > 1) {
+    if (!a.part || ws_bytes < p.nsplit * rows * (D + 2) * 4) return FOCR_EINVAL;
+    a.ml = (float2*)(a.part + p.nsplit * rows * D);
+  }
+  const long rmax = (long)a.max_q * a.group;
+  if (rmax <= 32) {
+    a.thin_rows = 32;
+    const long blocks = (long)p.nsplit * a.kv_heads * c.seqs;
+    if (blocks > INT32_MAX) return FOCR_EUNSUPPORTED;
+    if (rmax <= 16) hipLaunchKernelGGL((paged_thin_kernel<T, D, 1>), dim3(blocks), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((paged_thin_kernel<T, D, 2>), dim3(blocks), dim3(256), 0, st, a);
+    if (p.nsplit > 1) hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3(cdiv(rows, 4)), dim3(256), 0, st, a);
+  } else {
+    hipLaunchKernelGGL((paged_attention_row_kernel<T, D>), dim3(cdiv(rows, 4)), dim3(256), 0, st, a.q, a.ldt, a.ldh, a.kp, a.vp, c,
+                       a.o, a.ldto, a.ldho, a.max_q, a.heads, a.kv_heads, a.c2 * 0.6931471805599453f, a.causal);
+  }
+  return FOCR_OK;
 }
 
 extern "C" int focr_paged_attention_fwd(const void* q, long ldt, long ldh, const void* k_pages, const void* v_pages,
@@ -171,17 +701,25 @@ extern "C" int focr_paged_attention_fwd(const void* q, long ldt, long ldh, const
   PagedShape c;
   FOCR_CHECK_ARG(pg_shape(c, table, kv_lens, q_start, tokens, seqs, page, table_ld, num_pages, max_kv),
                  "page must be a power of two from 8 to 1024");
-  const dim3 grid((unsigned)((tokens * heads + 3) / 4));
-#define PG_ROW(T, DD)                                                                                                     \
-  hipLaunchKernelGGL((paged_attention_row_kernel<T, DD>), grid, dim3(256), 0, (hipStream_t)stream, (const T*)q, ldt, ldh,  \
-                     (const T*)k_pages, (const T*)v_pages, c, (T*)o, ldto, ldho, max_q, heads, kv_heads, scale, causal)
-#define PG_ROW_D(T)               \
-  if (dim == 64) PG_ROW(T, 64);   \
-  else if (dim == 128) PG_ROW(T, 128); \
-  else PG_ROW(T, 256)
-  if (dtype == FOCR_DT_F32) { PG_ROW_D(float); }
-  else if (dtype == FOCR_DT_BF16) { PG_ROW_D(bf16_t); }
-  else { PG_ROW_D(f16_t); }
+  int rc;
+  const bool wq = pg_aligned(q) && (((ldt | ldh) * pg_esize(dtype)) & 15) == 0;
+  const bool wo = pg_aligned(o) && (((ldto | ldho) * pg_esize(dtype)) & 15) == 0;
+#define PG_RUN(T, DD)                                                                                                       \
+  rc = pg_run<T, DD>(PgArgs<T>{(const T*)q, ldt, ldh, (const T*)k_pages, (const T*)v_pages, c, (T*)o, ldto, ldho, (float*)ws, \
+                               nullptr, max_q, heads, kv_heads, heads / kv_heads, 1, 0, causal ? 1 : 0, 0, wq, wo,             \
+                               scale * 1.4426950408889634f}, ws_bytes, dim, (hipStream_t)stream)
+#define PG_RUN_D(T)                    \
+  if (dim == 64) PG_RUN(T, 64);        \
+  else if (dim == 128) PG_RUN(T, 128); \
+  else PG_RUN(T, 256)
+  if (dtype == FOCR_DT_F32) { PG_RUN_D(float); }
+  else if (dtype == FOCR_DT_BF16) { PG_RUN_D(bf16_t); }
+  else { PG_RUN_D(f16_t); }
+  FOCR_CHECK_ARG(rc != FOCR_EINVAL, "workspace missing or too small (focr_paged_attention_ws_bytes)");
+  if (rc == FOCR_EUNSUPPORTED) {
+    focr_set_error("%s: too many sequences, heads and splits for one launch", __func__);
+    return rc;
+  }
   FOCR_LAUNCH_CHECK();
   return FOCR_OK;
 }
