@@ -276,7 +276,10 @@ __device__ __forceinline__ void pg_fill_nan(const PgArgs<T>& a, const PagedSeq& 
 // The next tile's loads go out between the two products.  MFMA time is a tenth of the bytes' (16-bit) to a third (fp32).
 // ======================================================================================================================
 #define PG_MAX_CHUNK 8192
-template <typename T, int D, int NT> constexpr int pg_thin_waves() { return D * NT <= 0 ? 4 : 1; }
+// queries that take 32 registers or more go through LDS: at most 256 registers keep two waves on a SIMD (one where the sums
+// of 32 rows x 256 alone take half of them)
+template <typename T, int D, int NT> constexpr bool pg_thin_q_lds() { return NT * D * sizeof(T) >= 512; }
+template <typename T, int D, int NT> constexpr int pg_thin_waves() { return NT * D <= 64 ? 4 : NT * D <= 256 ? 2 : 1; }
 template <typename T, int D, int NT>
 __global__ __launch_bounds__(256, (pg_thin_waves<T, D, NT>())) void paged_thin_kernel(PgArgs<T> a) {
   constexpr int ES = sizeof(T), EC = 16 / ES;          // elements of a chunk
@@ -287,10 +290,12 @@ __global__ __launch_bounds__(256, (pg_thin_waves<T, D, NT>())) void paged_thin_k
   __shared__ int pages[PG_MAX_CHUNK / 8 + 2];
   __shared__ float red[16 * NT * PITCH];
   __shared__ float2 wml[4][16 * NT];
+  constexpr bool QLDS = pg_thin_q_lds<T, D, NT>();
+  __shared__ u32x4 qs[QLDS ? NT * NU * 64 : 1];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, g = lane >> 4;
-  const int split = blockIdx.x % a.nsplit;
-  const int kh = blockIdx.x / a.nsplit % a.kv_heads, s = blockIdx.x / a.nsplit / a.kv_heads;
   const PagedShape& c = a.c;
+  // splits in the slowest place: blocks go round the 8 XCDs by number, and the last splits of most sequences are empty
+  const int kh = blockIdx.x % a.kv_heads, s = blockIdx.x / a.kv_heads % c.seqs, split = blockIdx.x / a.kv_heads / c.seqs;
   const PagedSeq sq = paged_seq(c, s);
   if ((long)sq.n * a.group > a.thin_rows && sq.n <= a.max_q) return;     // the other kernel's
   if (sq.n == 0) return;
@@ -313,9 +318,8 @@ __global__ __launch_bounds__(256, (pg_thin_waves<T, D, NT>())) void paged_thin_k
     any_bad |= p < 0;
     pages[i] = p < 0 ? 0 : p;
   }
-  any_bad = __syncthreads_or(any_bad);
 
-  u32x4 qf[NT][NU];
+  u32x4 qf[QLDS ? 1 : NT][QLDS ? 1 : NU];
   int vis[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
@@ -325,8 +329,18 @@ __global__ __launch_bounds__(256, (pg_thin_waves<T, D, NT>())) void paged_thin_k
     vis[t] = ok ? paged_visible(sq.len, sq.n, i, a.causal) : 0;
     const T* p = a.q + (sq.t0 + i) * a.ldt + h * a.ldh + g * EC;
 #pragma unroll
-    for (int u = 0; u < NU; ++u) qf[t][u] = ok ? pg_load_chunk(p + u * 4 * EC, a.wide_q) : u32x4{0, 0, 0, 0};
+    for (int u = 0; u < NU; ++u) {
+      if (QLDS && (u & 3) != wave) continue;
+      const u32x4 x = ok ? pg_load_chunk(p + u * 4 * EC, a.wide_q) : u32x4{0, 0, 0, 0};
+      if constexpr (QLDS) qs[(t * NU + u) * 64 + lane] = x;
+      else qf[t][u] = x;
+    }
   }
+  any_bad = __syncthreads_or(any_bad);
+  auto q_chunk = [&](int t, int u) {
+    if constexpr (QLDS) return qs[(t * NU + u) * 64 + lane];
+    else return qf[t][u];
+  };
 
   const long head_bytes = ((long)D * ES) << c.page_shift, page_bytes = head_bytes * a.kv_heads;
   const char *kbase = (const char*)a.kp + kh * head_bytes, *vbase = (const char*)a.vp + kh * head_bytes;
@@ -406,7 +420,7 @@ __global__ __launch_bounds__(256, (pg_thin_waves<T, D, NT>())) void paged_thin_k
       for (int sub = 0; sub < KT / 16; ++sub) {
         sc[t][sub] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int u = 0; u < NU; ++u) sc[t][sub] = PgMma<T>::mma16(kr[sub][u], qf[t][u], sc[t][sub]);
+        for (int u = 0; u < NU; ++u) sc[t][sub] = PgMma<T>::mma16(kr[sub][u], q_chunk(t, u), sc[t][sub]);
       }
     if (next < k1) load_k(next);
     if (base + KT > vmin) {
@@ -505,6 +519,7 @@ __global__ __launch_bounds__(256, (pg_thin_waves<T, D, NT>())) void paged_thin_k
         const u32x4 vf = v_frag(u, e);
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[t][u][e] = PgMma<T>::mma16(vf, pf[t], acc[t][u][e]);
+        if (NT * D >= 256 && (e & 1)) __builtin_amdgcn_sched_barrier(0);       // no more transposed chunks ahead than registers
       }
     if (next < k1) load_v(next);
   }
@@ -565,32 +580,49 @@ __global__ __launch_bounds__(256, (pg_thin_waves<T, D, NT>())) void paged_thin_k
   }
 }
 
-// ---- joins the splits of a row: one wave per (token, head) --------------------------------------------------------------
+// ---- joins the splits of a row: one block per (token, head), the splits dealt out to its 4 waves ------------------------
 template <typename T, int D>
 __global__ __launch_bounds__(256) void paged_join_kernel(PgArgs<T> a) {
   constexpr int E = D / 64;
-  const int lane = threadIdx.x & 63;
-  const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= a.c.tokens * a.heads) return;
-  const long t = row / a.heads;
+  __shared__ float wmax[4], wsum[4], acc[3][D];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long row = blockIdx.x, t = row / a.heads;
   const int h = (int)(row - t * a.heads), s = pg_seq_of_row(a.c, t, lane);
   const PagedSeq sq = paged_seq(a.c, s);
   const long i = t - sq.t0;
   if (i < 0 || i >= sq.n || sq.bad || sq.n > a.max_q || sq.len <= a.chunk) return;
   const int n = (paged_visible(sq.len, sq.n, (int)i, a.causal) + a.chunk - 1) / a.chunk;
   const long step = a.c.tokens * a.heads;
-  float mx = -INFINITY, ls = 0.f, v[E];
+  float mx = -INFINITY;
+  for (int k = threadIdx.x; k < n; k += 256) mx = fmaxf(mx, a.ml[row + k * step].x);
+  mx = wave_max(mx);
+  if (lane == 0) wmax[wave] = mx;
+  __syncthreads();
+  mx = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
+  float ls = 0.f, v[E];
+#pragma unroll
   for (int e = 0; e < E; ++e) v[e] = 0.f;
-  for (int k = 0; k < n; ++k) mx = fmaxf(mx, a.ml[row + k * step].x);
-  for (int k = 0; k < n; ++k) {
+#pragma unroll 4
+  for (int k = wave; k < n; k += 4) {
     const float2 ml = a.ml[row + k * step];
     const float w = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mx);
     ls += pg_share(ml.y, ml.x - mx);
     const float* p = a.part + (row + k * step) * D + lane * E;
+#pragma unroll
     for (int e = 0; e < E; ++e) v[e] += w * p[e];
   }
+  if (lane == 0) wsum[wave] = ls;
+  if (wave)
+    for (int e = 0; e < E; ++e) acc[wave - 1][lane * E + e] = v[e];
+  __syncthreads();
+  if (wave) return;
+  ls = wsum[0] + wsum[1] + wsum[2] + wsum[3];
   T* o = a.o + t * a.ldto + h * a.ldho + lane * E;
-  for (int e = 0; e < E; ++e) o[e] = (T)(ls == 0.f ? 0.f : v[e] / ls);
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const float x = v[e] + acc[0][lane * E + e] + acc[1][lane * E + e] + acc[2][lane * E + e];
+    o[e] = (T)(ls == 0.f ? 0.f : x / ls);
+  }
 }
 
 // ---- C entries ---------------------------------------------------------------------------------------------------------
@@ -631,24 +663,23 @@ extern "C" int focr_paged_append(const void* k_new, const void* v_new, long ldtk
   return FOCR_OK;
 }
 
-// Splits of the key axis.  The keys of a (sequence, key head) go to blocks of `chunk` keys each, enough of them to fill the 256
-// CUs several times over even when most sequences are far shorter than the bound max_kv; a sequence of at most `chunk` keys
-// writes its output directly, the parts of a longer one are joined by a second launch.
+// Splits of the key axis.  The keys of a (sequence, key head) go to blocks of `chunk` keys; a sequence of at most `chunk` keys
+// writes its output directly, the parts of a longer one are joined by a second launch.  Up to 4096 blocks, so that sequences
+// of very different lengths still fill the card evenly (64 sequences of 100 .. 8190 tokens x 8 heads, bf16, 128 wide: 2048
+// blocks 198 us, 4096 193 us, 8192 200 us), but no fewer than 1024 keys in a block while there are blocks enough for two on each
+// CU: a block's start and end cost as much as some hundred keys (2 sequences of 131k: 1024 keys 205 us, 512 224 us, 256 254 us).
 struct PgPlan {
   int nsplit, chunk;
 };
-#ifndef PG_TARGET
-#define PG_TARGET 2048
-#endif
-#ifndef PG_MINCHUNK
-#define PG_MINCHUNK 256
-#endif
 static PgPlan pg_plan(int seqs, int kv_heads, int max_kv) {
-  const long groups = (long)seqs * kv_heads;
-  const long want = groups >= PG_TARGET ? 1 : (PG_TARGET + groups - 1) / groups;
+  const long groups = (long)seqs * kv_heads, want = (4096 + groups - 1) / groups;
   long chunk = (max_kv + want - 1) / want;
+  if (chunk < 1024) chunk = 1024;
+  if (groups * ((max_kv + chunk - 1) / chunk) < 512) {
+    chunk = max_kv * groups / 512;
+    chunk = chunk < 256 ? 256 : chunk > 1024 ? 1024 : chunk;
+  }
   chunk = (chunk + 127) / 128 * 128;
-  if (chunk < PG_MINCHUNK) chunk = PG_MINCHUNK;
   if (chunk > PG_MAX_CHUNK) chunk = PG_MAX_CHUNK;
   const int n = (int)((max_kv + chunk - 1) / chunk);
   return {n > 0 ? n : 1, (int)chunk};
@@ -679,7 +710,7 @@ static int pg_run(PgArgs<T> a, long ws_bytes, int dim, hipStream_t st) {
     if (blocks > INT32_MAX) return FOCR_EUNSUPPORTED;
     if (rmax <= 16) hipLaunchKernelGGL((paged_thin_kernel<T, D, 1>), dim3(blocks), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((paged_thin_kernel<T, D, 2>), dim3(blocks), dim3(256), 0, st, a);
-    if (p.nsplit > 1) hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3(cdiv(rows, 4)), dim3(256), 0, st, a);
+    if (p.nsplit > 1) hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3((unsigned)rows), dim3(256), 0, st, a);
   } else {
     hipLaunchKernelGGL((paged_attention_row_kernel<T, D>), dim3(cdiv(rows, 4)), dim3(256), 0, st, a.q, a.ldt, a.ldh, a.kp, a.vp, c,
                        a.o, a.ldto, a.ldho, a.max_q, a.heads, a.kv_heads, a.c2 * 0.6931471805599453f, a.causal);
