@@ -9,10 +9,6 @@
 typedef _Float16 f16_t;
 typedef __bf16 bf16_t;
 
-__device__ __forceinline__ float pg_to_f(float x) { return x; }
-__device__ __forceinline__ float pg_to_f(bf16_t x) { return (float)x; }
-__device__ __forceinline__ float pg_to_f(f16_t x) { return (float)x; }
-
 // the last i in [0, n) with f(i) <= key, for a non-decreasing f with f(0) <= key (64 probes a round; all lanes take part)
 template <typename F>
 __device__ __forceinline__ int pg_find(F f, int n, long key, int lane) {
@@ -67,51 +63,6 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const char* __restric
       *(uint16_t*)(vp + dst) = *(const uint16_t*)vs;
     }
   }
-}
-
-// ---- attention, the plainest form: one wave per (token, head), the head's dimensions across the lanes -----------------
-template <typename T, int D>
-__global__ __launch_bounds__(256) void paged_attention_row_kernel(const T* __restrict__ q, long ldt, long ldh,
-                                                                  const T* __restrict__ kp, const T* __restrict__ vp,
-                                                                  PagedShape c, T* __restrict__ o, long ldto, long ldho,
-                                                                  int max_q, int heads, int kv_heads, float scale, int causal) {
-  constexpr int E = D / 64;
-  const int lane = threadIdx.x & 63;
-  const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= c.tokens * heads) return;
-  const long t = row / heads;
-  const int h = (int)(row - t * heads), kh = h / (heads / kv_heads);
-  const int s = pg_seq_of_row(c, t, lane);
-  const PagedSeq sq = paged_seq(c, s);
-  const long i = t - sq.t0;
-  if (i < 0 || i >= sq.n) return;
-  bool bad = sq.bad || sq.n > max_q;
-  float qv[E], acc[E];
-  for (int e = 0; e < E; ++e) {
-    qv[e] = pg_to_f(q[t * ldt + h * ldh + e * 64 + lane]) * scale;
-    acc[e] = 0.f;
-  }
-  float m = -INFINITY, l = 0.f;
-  const int vis = bad ? 0 : paged_visible(sq.len, sq.n, (int)i, causal);
-  for (int j = 0; j < vis; ++j) {
-    const int pg = paged_page(c, s, j);
-    if (pg < 0) {
-      bad = true;
-      break;
-    }
-    const long at = ((((long)pg * kv_heads + kh) << c.page_shift) + (j & ((1 << c.page_shift) - 1))) * D + lane;
-    float d = 0.f;
-    for (int e = 0; e < E; ++e) d = fmaf(qv[e], pg_to_f(kp[at + e * 64]), d);
-    d = wave_sum(d);
-    const float mn = fmaxf(m, d);
-    const float base = mn == -INFINITY ? 0.f : mn;
-    const float a = expf(m - base), p = expf(d - base);
-    m = mn;
-    l = l * a + p;
-    for (int e = 0; e < E; ++e) acc[e] = acc[e] * a + p * pg_to_f(vp[at + e * 64]);
-  }
-  for (int e = 0; e < E; ++e)
-    o[t * ldto + h * ldho + e * 64 + lane] = (T)(bad ? NAN : l == 0.f ? 0.f : acc[e] / l);
 }
 
 // ---- matrix instructions -----------------------------------------------------------------------------------------------
@@ -217,7 +168,7 @@ struct PgArgs {
   long ldto, ldho;
   float* part;   // [split][token][head][D], weights relative to the split's own maximum
   float2* ml;    // [split][token][head]: that maximum (in log2 units) and the sum of the weights
-  int max_q, heads, kv_heads, group, nsplit, chunk, causal, thin_rows, wide_q, wide_o;
+  int max_q, heads, kv_heads, group, nsplit, chunk, tile_chunk, causal, thin_rows, wide_q, wide_o;
   float c2;      // scale * log2(e)
 };
 
@@ -580,6 +531,320 @@ __global__ __launch_bounds__(256, (pg_thin_waves<T, D, NT>())) void paged_thin_k
   }
 }
 
+// ======================================================================================================================
+// Many rows (a chunk's tokens x the heads that share a key head, flattened: a block takes 32 NQ NW neighbouring rows, so one
+// staged tile of keys serves every head of the group): bound by the matrix instructions.  32 x 32 tiles in the same
+// orientation as above -- S^T = K Q^T leaves a lane one query column, whose weights are B of O^T = V^T P^T as they stand -- with
+// KT keys and values at a time in LDS, double-buffered by direct loads, 16-byte chunks XOR-swizzled by row so that both the
+// row-wise reads of K and the transposing reads of V (ds_read_b64_tr_b16; plain words in fp32) use every bank.  A wave skips
+// the tiles that none of its rows sees and compares positions only where its rows differ.
+// ======================================================================================================================
+template <int CPR> __device__ __forceinline__ int pg_swz(int row) {
+  if constexpr (CPR == 8) return ((row >> 1 & 1) << 2) | ((row >> 2 & 1) << 1) | (row >> 3 & 1);
+  else return ((row & 7) << 1) | (row >> 3 & 1);
+}
+typedef __attribute__((ext_vector_type(4))) short pg_s16x4;
+__device__ __forceinline__ uint2 pg_read_tr(const char* p) {
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pg_s16x4*)p));
+}
+
+template <typename T, int D, int NQ> constexpr int pg_tile_waves() { return NQ * D * sizeof(T) <= 512 ? 2 : 1; }
+template <typename T, int D, int NQ, int NW>
+__global__ __launch_bounds__(64 * NW, (pg_tile_waves<T, D, NQ>())) void paged_tile_kernel(PgArgs<T> a) {
+  constexpr int ES = sizeof(T), EC = 16 / ES, ROWB = D * ES, CPR = ROWB / 16;
+  constexpr int KT = ROWB <= 256 ? 64 : 32, NS = KT / 32;
+  constexpr int NU = ROWB / 32;                        // contraction steps of S^T (pairs of chunks)
+  constexpr int RPI = 64 / CPR;                        // rows one direct load of a wave brings
+  constexpr int NL = KT / (RPI * NW);                  // such loads per wave, for K and for V
+  constexpr int DT = D / 32, PT = ES == 4 ? 4 : 2;     // O^T tiles; contraction steps of O^T per 32 keys
+  constexpr int ROWS = 32 * NQ * NW;
+  extern __shared__ __attribute__((aligned(128))) char pg_smem[];
+  char* const ksm = pg_smem;                           // [2][KT][ROWB]
+  char* const vsm = pg_smem + 2 * KT * ROWB;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l32 = lane & 31, hh = lane >> 5;
+  const PagedShape& c = a.c;
+  const long tiles = paged_tiles(c.tokens, c.seqs, a.group, ROWS);
+  const int kh = blockIdx.x % a.kv_heads;
+  const long ti = tiles - 1 - blockIdx.x / a.kv_heads % tiles;          // the tiles with the most keys first
+  const int split = (int)(blockIdx.x / a.kv_heads / tiles);
+  int s;
+  if (c.q_start) {
+    const int* qs = c.q_start;
+    const int grp = a.group;
+    s = pg_find([=](int i) { return paged_first_tile(qs[i], i, grp, ROWS); }, c.seqs, ti, lane);
+  } else {
+    const long n = c.tokens / c.seqs, grp = a.group;
+    s = pg_find([=](int i) { return paged_first_tile(i * n, i, (int)grp, ROWS); }, c.seqs, ti, lane);
+  }
+  const PagedSeq sq = paged_seq(c, s);
+  const long R = (long)sq.n * a.group, r0 = (ti - paged_first_tile(sq.t0, s, a.group, ROWS)) * ROWS;
+  if (r0 < 0 || r0 >= R || R <= a.thin_rows) return;
+  if (sq.bad || sq.n > a.max_q) {
+    if (split == 0)
+      for (long x = tid; x < ROWS * D; x += 64 * NW) {
+        const long r = r0 + x / D;
+        if (r < R) a.o[(sq.t0 + r / a.group) * a.ldto + (kh * a.group + r % a.group) * a.ldho + x % D] = (T)NAN;
+      }
+    return;
+  }
+  const int tok0 = (int)(r0 / a.group), tok1 = (int)((R < r0 + ROWS ? R - 1 : r0 + ROWS - 1) / a.group);
+  const int vmin = paged_visible(sq.len, sq.n, tok0, a.causal), kend = paged_visible(sq.len, sq.n, tok1, a.causal);
+  const bool direct = sq.len <= a.tile_chunk;
+  const int k0 = split * a.tile_chunk;
+  if (split && k0 >= kend) return;
+  const int k1 = kend < k0 + a.tile_chunk ? kend : k0 + a.tile_chunk;
+  const int nt = k1 > k0 ? (k1 - k0 + KT - 1) / KT : 0;
+
+  // this wave's rows: one query column per lane
+  u32x4 qf[NQ][NU];
+  int vis[NQ], wvmin = INT32_MAX, wvmax = 0;
+#pragma unroll
+  for (int t = 0; t < NQ; ++t) {
+    const long r = r0 + (wave * NQ + t) * 32 + l32;
+    const bool ok = r < R;
+    const long i = ok ? r / a.group : 0;
+    const int h = kh * a.group + (ok ? (int)(r - i * a.group) : 0);
+    vis[t] = ok ? paged_visible(sq.len, sq.n, (int)i, a.causal) : 0;
+    if (ok) {
+      wvmin = vis[t] < wvmin ? vis[t] : wvmin;
+      wvmax = vis[t] > wvmax ? vis[t] : wvmax;
+    }
+    const T* p = a.q + (sq.t0 + i) * a.ldt + h * a.ldh + hh * EC;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) qf[t][u] = ok ? pg_load_chunk(p + u * 2 * EC, a.wide_q) : u32x4{0, 0, 0, 0};
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const int x = __shfl_xor(wvmin, o, 64), y = __shfl_xor(wvmax, o, 64);
+    wvmin = x < wvmin ? x : wvmin;
+    wvmax = y > wvmax ? y : wvmax;
+  }
+  wvmin = __builtin_amdgcn_readfirstlane(wvmin);
+  wvmax = __builtin_amdgcn_readfirstlane(wvmax);
+
+  const long head_bytes = (long)ROWB << c.page_shift, page_bytes = head_bytes * a.kv_heads;
+  const char *kbase = (const char*)a.kp + kh * head_bytes, *vbase = (const char*)a.vp + kh * head_bytes;
+  const int slot_mask = (1 << c.page_shift) - 1;
+  const int* trow = c.table + (long)s * c.table_ld;
+  int pg[NL];
+  bool bad_page = false;
+  auto key_of = [&](int base, int i) {                 // key this lane brings in load i; past the end: the last one again
+    const int k = base + (i * NW + wave) * RPI + lane / CPR;
+    return k < k1 ? k : k1 - 1;
+  };
+  auto find_pages = [&](int base) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) pg[i] = trow[key_of(base, i) >> c.page_shift];
+  };
+  auto stage = [&](int base, int buf) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int row = (i * NW + wave) * RPI + lane / CPR;
+      const bool ok = pg[i] >= 0 && pg[i] < c.num_pages;
+      bad_page |= !ok;
+      const long at = (ok ? pg[i] : 0) * page_bytes + (long)(key_of(base, i) & slot_mask) * ROWB
+                      + (((lane % CPR) ^ pg_swz<CPR>(row)) * 16);
+      const int dst = buf * KT * ROWB + (i * NW + wave) * 1024;
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(kbase + at),
+                                       (__attribute__((address_space(3))) void*)(ksm + dst), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(vbase + at),
+                                       (__attribute__((address_space(3))) void*)(vsm + dst), 16, 0, 0);
+    }
+  };
+  // A operand of O^T: 32 values d of the keys sub * 32 + step * (32 / PT) ..
+  auto v_frag = [&](const char* v, int sub, int step, int dt) {
+    u32x4 r;
+    if constexpr (ES == 4) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int row = sub * 32 + step * 8 + hh * 4 + e, d = dt * 32 + l32;
+        r[e] = *(const uint32_t*)(v + row * ROWB + (((d >> 2) ^ pg_swz<CPR>(row)) << 4) + (d & 3) * 4);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = sub * 32 + step * 16 + e * 8 + hh * 4 + (lane >> 2 & 3);
+        const int col = (dt * 32 + (lane >> 4 & 1) * 16 + (lane & 3) * 4) * 2;
+        const uint2 x = pg_read_tr(v + row * ROWB + (((col >> 4) ^ pg_swz<CPR>(row)) << 4) + (col & 15));
+        r[2 * e] = x.x;
+        r[2 * e + 1] = x.y;
+      }
+    }
+    return r;
+  };
+
+  f32x16 acc[NQ][DT];
+  float m[NQ], l[NQ];
+#pragma unroll
+  for (int t = 0; t < NQ; ++t) {
+    m[t] = -INFINITY;
+    l[t] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) acc[t][dt] = f32x16{0};
+  }
+  if (nt) {
+    find_pages(k0);
+    stage(k0, 0);
+    find_pages(k0 + KT < k1 ? k0 + KT : k0);
+  }
+  for (int it = 0; it < nt; ++it) {
+    const int base = k0 + it * KT, buf = it & 1;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();                                   // this tile is there; everyone is done with the other buffer
+    if (it + 1 < nt) {
+      stage(base + KT, buf ^ 1);
+      find_pages(base + 2 * KT < k1 ? base + 2 * KT : k0);
+    }
+    const char *kt = ksm + buf * KT * ROWB, *vt = vsm + buf * KT * ROWB;
+    if (base + KT > vmin) {                            // some row of the block does not see all of this tile: 0 * inf
+      bool odd = false;
+      char* mine = (char*)vt + tid * 16;
+#pragma unroll
+      for (int i = 0; i < KT * ROWB / (1024 * NW); ++i) {
+        const u32x4 x = *(const u32x4*)(mine + i * 1024 * NW);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) odd |= pg_finite<T>(x[w]) != x[w];
+      }
+      if (__syncthreads_or(odd)) {
+        // what the infinities and NaN of the tile add to the rows that see them; then they leave the tile
+#pragma unroll 1
+        for (int sub = 0; sub < NS; ++sub)
+#pragma unroll 1
+          for (int step = 0; step < PT; ++step)
+#pragma unroll
+            for (int t = 0; t < NQ; ++t) {
+              u32x4 see;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                if constexpr (ES == 4) see[j] = base + sub * 32 + step * 8 + hh * 4 + j < vis[t] ? PgMma<T>::ONE : 0u;
+                else {
+                  const int key = base + sub * 32 + step * 16 + (j >> 1) * 8 + hh * 4 + (2 * j & 3);
+                  see[j] = (key < vis[t] ? PgMma<T>::ONE : 0u) | (key + 1 < vis[t] ? PgMma<T>::ONE << 16 : 0u);
+                }
+              }
+#pragma unroll
+              for (int dt = 0; dt < DT; ++dt) {
+                const u32x4 vf = v_frag(vt, sub, step, dt);
+                const f32x16 z = {0};
+                const f32x16 pos = PgMma<T>::mma32(pg_class<T, 1>(vf), see, z);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[t][dt][i] = pg_with_nonfinite(acc[t][dt][i], pos[i], 0.f, 0.f);
+                const f32x16 neg = PgMma<T>::mma32(pg_class<T, 2>(vf), see, z);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[t][dt][i] = pg_with_nonfinite(acc[t][dt][i], 0.f, neg[i], 0.f);
+                const f32x16 nan = PgMma<T>::mma32(pg_class<T, 3>(vf), see, z);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[t][dt][i] = pg_with_nonfinite(acc[t][dt][i], 0.f, 0.f, nan[i]);
+                __builtin_amdgcn_sched_barrier(0);
+              }
+            }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < KT * ROWB / (1024 * NW); ++i) {
+          u32x4 x = *(const u32x4*)(mine + i * 1024 * NW);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) x[w] = pg_finite<T>(x[w]);
+          *(u32x4*)(mine + i * 1024 * NW) = x;
+        }
+        __syncthreads();
+      }
+    }
+    if (base >= wvmax) continue;                       // nothing here for this wave's rows
+    f32x16 sc[NQ][NS];
+#pragma unroll
+    for (int sub = 0; sub < NS; ++sub) {
+#pragma unroll
+      for (int t = 0; t < NQ; ++t) sc[t][sub] = f32x16{0};
+      const int row = sub * 32 + l32;
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
+        const u32x4 kf = *(const u32x4*)(kt + row * ROWB + (((2 * u + hh) ^ pg_swz<CPR>(row)) << 4));
+#pragma unroll
+        for (int t = 0; t < NQ; ++t) sc[t][sub] = PgMma<T>::mma32(kf, qf[t][u], sc[t][sub]);
+      }
+    }
+    if (base + KT > wvmin) {
+#pragma unroll
+      for (int t = 0; t < NQ; ++t)
+#pragma unroll
+        for (int sub = 0; sub < NS; ++sub)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (base + sub * 32 + 8 * (i >> 2) + 4 * hh + (i & 3) >= vis[t]) sc[t][sub][i] = -INFINITY;
+    }
+    u32x4 pf[NQ][NS][PT];
+#pragma unroll
+    for (int t = 0; t < NQ; ++t) {
+      float mx = m[t];
+#pragma unroll
+      for (int sub = 0; sub < NS; ++sub)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[t][sub][i]);
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float ref = mx == -INFINITY ? 0.f : mx * a.c2;
+      if (__any(mx > m[t])) {
+        const float al = __builtin_amdgcn_exp2f(m[t] * a.c2 - ref);
+        l[t] *= al;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) acc[t][dt] *= al;
+        m[t] = mx;
+      }
+#pragma unroll
+      for (int sub = 0; sub < NS; ++sub) {
+        float p[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          p[i] = __builtin_amdgcn_exp2f(fmaf(sc[t][sub][i], a.c2, -ref));
+          l[t] += p[i];
+        }
+#pragma unroll
+        for (int step = 0; step < PT; ++step)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if constexpr (ES == 4) pf[t][sub][step][j] = __float_as_uint(p[step * 4 + j]);
+            else pf[t][sub][step][j] = pg_pack<T>(p[step * 8 + 2 * j], p[step * 8 + 2 * j + 1]);
+          }
+      }
+    }
+#pragma unroll
+    for (int sub = 0; sub < NS; ++sub)
+#pragma unroll
+      for (int step = 0; step < PT; ++step)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          const u32x4 vf = v_frag(vt, sub, step, dt);
+#pragma unroll
+          for (int t = 0; t < NQ; ++t) acc[t][dt] = PgMma<T>::mma32(vf, pf[t][sub][step], acc[t][dt]);
+        }
+  }
+  const bool any_bad = __syncthreads_or(bad_page);
+
+  // out: lane = row, four neighbouring values d = 32 dt + 8 q + 4 (l / 32) + ..
+#pragma unroll
+  for (int t = 0; t < NQ; ++t) {
+    const long r = r0 + (wave * NQ + t) * 32 + l32;
+    float ls = l[t] + __shfl_xor(l[t], 32, 64);
+    if (any_bad) ls = NAN;
+    if (r >= R) continue;
+    const long i = r / a.group;
+    const int h = kh * a.group + (int)(r - i * a.group);
+    const float inv = direct ? (ls == 0.f ? 0.f : 1.f / ls) : 1.f;
+    T* o = a.o + (sq.t0 + i) * a.ldto + h * a.ldho + 4 * hh;
+    const long row = ((long)split * c.tokens + sq.t0 + i) * a.heads + h;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = ls == 0.f ? 0.f : acc[t][dt][4 * q + e] * inv;
+        if (direct) pg_store_row<T, 4>(o + dt * 32 + q * 8, v, a.wide_o);
+        else *(f32x4*)(a.part + row * D + dt * 32 + q * 8 + 4 * hh) = f32x4{v[0], v[1], v[2], v[3]};
+      }
+    if (!direct && hh == 0) a.ml[row] = float2{any_bad ? 0.f : m[t] * a.c2, ls};
+  }
+}
+
 // ---- joins the splits of a row: one block per (token, head), the splits dealt out to its 4 waves ------------------------
 template <typename T, int D>
 __global__ __launch_bounds__(256) void paged_join_kernel(PgArgs<T> a) {
@@ -590,8 +855,9 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PgArgs<T> a) {
   const int h = (int)(row - t * a.heads), s = pg_seq_of_row(a.c, t, lane);
   const PagedSeq sq = paged_seq(a.c, s);
   const long i = t - sq.t0;
-  if (i < 0 || i >= sq.n || sq.bad || sq.n > a.max_q || sq.len <= a.chunk) return;
-  const int n = (paged_visible(sq.len, sq.n, (int)i, a.causal) + a.chunk - 1) / a.chunk;
+  const int chunk = (long)sq.n * a.group <= a.thin_rows ? a.chunk : a.tile_chunk;
+  if (i < 0 || i >= sq.n || sq.bad || sq.n > a.max_q || sq.len <= chunk) return;
+  const int n = (paged_visible(sq.len, sq.n, (int)i, a.causal) + chunk - 1) / chunk;
   const long step = a.c.tokens * a.heads;
   float mx = -INFINITY;
   for (int k = threadIdx.x; k < n; k += 256) mx = fmaxf(mx, a.ml[row + k * step].x);
@@ -669,52 +935,93 @@ extern "C" int focr_paged_append(const void* k_new, const void* v_new, long ldtk
 // blocks 198 us, 4096 193 us, 8192 200 us), but no fewer than 1024 keys in a block while there are blocks enough for two on each
 // CU: a block's start and end cost as much as some hundred keys (2 sequences of 131k: 1024 keys 205 us, 512 224 us, 256 254 us).
 struct PgPlan {
-  int nsplit, chunk;
+  int thin_rows;           // sequences of at most this many rows go to the thin kernel, the rest to the tiles
+  int nsplit, chunk;       // of the thin kernel
+  int tsplit, tile_chunk;  // of the tiles
 };
-static PgPlan pg_plan(int seqs, int kv_heads, int max_kv) {
-  const long groups = (long)seqs * kv_heads, want = (4096 + groups - 1) / groups;
-  long chunk = (max_kv + want - 1) / want;
-  if (chunk < 1024) chunk = 1024;
-  if (groups * ((max_kv + chunk - 1) / chunk) < 512) {
-    chunk = max_kv * groups / 512;
-    chunk = chunk < 256 ? 256 : chunk > 1024 ? 1024 : chunk;
+#ifndef PGNQ
+#define PGNQ 1
+#define PGNW 4
+#endif
+template <typename T, int D> constexpr int pg_tile_rows() { return 32 * PGNQ * PGNW; }
+static PgPlan pg_plan(long tokens, int seqs, int kv_heads, int group, int max_q, int max_kv, bool ragged) {
+  PgPlan p = {0, 1, 128, 1, INT32_MAX};
+  const long rmax = (long)max_q * group;
+  if (rmax <= 32) p.thin_rows = rmax <= 16 ? 16 : 32;
+  else if (ragged) p.thin_rows = group <= 16 ? 16 : group <= 32 ? 32 : 0;
+  if (p.thin_rows) {
+    const long groups = (long)seqs * kv_heads, want = (4096 + groups - 1) / groups;
+    long chunk = (max_kv + want - 1) / want;
+    if (chunk < 1024) chunk = 1024;
+    if (groups * ((max_kv + chunk - 1) / chunk) < 512) {
+      chunk = max_kv * groups / 512;
+      chunk = chunk < 256 ? 256 : chunk > 1024 ? 1024 : chunk;
+    }
+    chunk = (chunk + 127) / 128 * 128;
+    if (chunk > PG_MAX_CHUNK) chunk = PG_MAX_CHUNK;
+    const int n = (int)((max_kv + chunk - 1) / chunk);
+    p.nsplit = n > 0 ? n : 1;
+    p.chunk = (int)chunk;
   }
-  chunk = (chunk + 127) / 128 * 128;
-  if (chunk > PG_MAX_CHUNK) chunk = PG_MAX_CHUNK;
-  const int n = (int)((max_kv + chunk - 1) / chunk);
-  return {n > 0 ? n : 1, (int)chunk};
+  if (rmax > 32) {
+    const long blocks = (tokens * group + 127) / 128 * kv_heads;
+    if (blocks < 512 && max_kv > 512) {
+      long chunk = max_kv * blocks / 512;
+      chunk = ((chunk < 512 ? 512 : chunk) + 127) / 128 * 128;
+      p.tsplit = (int)((max_kv + chunk - 1) / chunk);
+      p.tile_chunk = (int)chunk;
+    }
+  }
+  return p;
+}
+static long pg_ws_bytes(const PgPlan& p, long rows, int dim) {
+  const long n = p.nsplit > p.tsplit ? p.nsplit : p.tsplit;
+  return n == 1 ? 0 : n * rows * (dim + 2) * 4;
 }
 
+// the larger of the two forms (one or several row counts per call) is asked for
 extern "C" long focr_paged_attention_ws_bytes(long tokens, int seqs, int heads, int kv_heads, int dim, int max_q, int max_kv,
                                               int dtype) {
-  if (tokens <= 0 || seqs <= 0 || heads <= 0 || kv_heads <= 0 || dim <= 0 || max_q < 0 || max_kv < 0) return tokens == 0 || seqs == 0 ? 0 : -1;
-  const PgPlan p = pg_plan(seqs, kv_heads, max_kv);
-  return p.nsplit == 1 ? 0 : p.nsplit * tokens * heads * (dim + 2) * 4;
+  if (tokens == 0 || seqs == 0) return 0;
+  if (tokens < 0 || seqs < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || dim <= 0 || max_q < 0 || max_kv < 0) return -1;
+  const int group = heads / kv_heads;
+  const long a = pg_ws_bytes(pg_plan(tokens, seqs, kv_heads, group, max_q, max_kv, false), tokens * heads, dim);
+  const long b = pg_ws_bytes(pg_plan(tokens, seqs, kv_heads, group, max_q, max_kv, true), tokens * heads, dim);
+  return a > b ? a : b;
 }
 
 template <typename T, int D>
-static int pg_run(PgArgs<T> a, long ws_bytes, int dim, hipStream_t st) {
+static int pg_run(PgArgs<T> a, long ws_bytes, hipStream_t st) {
   const PagedShape& c = a.c;
-  const PgPlan p = pg_plan(c.seqs, a.kv_heads, c.max_kv);
+  const PgPlan p = pg_plan(c.tokens, c.seqs, a.kv_heads, a.group, a.max_q, c.max_kv, c.q_start != nullptr);
   a.nsplit = p.nsplit;
   a.chunk = p.chunk;
-  const long rows = c.tokens * a.heads;
-  if (p.nsplit > 1) {
-    if (!a.part || ws_bytes < p.nsplit * rows * (D + 2) * 4) return FOCR_EINVAL;
-    a.ml = (float2*)(a.part + p.nsplit * rows * D);
+  a.tile_chunk = p.tile_chunk;
+  a.thin_rows = p.thin_rows;
+  const long rows = c.tokens * a.heads, need = pg_ws_bytes(p, rows, D);
+  if (need) {
+    if (!a.part || ws_bytes < need) return FOCR_EINVAL;
+    a.ml = (float2*)(a.part + need / ((D + 2) * 4) * D);
   }
   const long rmax = (long)a.max_q * a.group;
-  if (rmax <= 32) {
-    a.thin_rows = 32;
-    const long blocks = (long)p.nsplit * a.kv_heads * c.seqs;
-    if (blocks > INT32_MAX) return FOCR_EUNSUPPORTED;
-    if (rmax <= 16) hipLaunchKernelGGL((paged_thin_kernel<T, D, 1>), dim3(blocks), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((paged_thin_kernel<T, D, 2>), dim3(blocks), dim3(256), 0, st, a);
-    if (p.nsplit > 1) hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3((unsigned)rows), dim3(256), 0, st, a);
-  } else {
-    hipLaunchKernelGGL((paged_attention_row_kernel<T, D>), dim3(cdiv(rows, 4)), dim3(256), 0, st, a.q, a.ldt, a.ldh, a.kp, a.vp, c,
-                       a.o, a.ldto, a.ldho, a.max_q, a.heads, a.kv_heads, a.c2 * 0.6931471805599453f, a.causal);
+  const long thin = (long)p.nsplit * a.kv_heads * c.seqs;
+  const long tiles = paged_tiles(c.tokens, c.seqs, a.group, pg_tile_rows<T, D>()) * a.kv_heads * p.tsplit;
+  if (thin > INT32_MAX || tiles > INT32_MAX || rows > INT32_MAX) return FOCR_EUNSUPPORTED;
+  if (rmax > 32) {
+    constexpr int LDS = 4 * (D * sizeof(T) <= 256 ? 64 : 32) * D * sizeof(T);
+    auto kern = paged_tile_kernel<T, D, PGNQ, PGNW>;
+    if (LDS > 49152) {
+      static focr_dev_flags done;
+      if (focr_dev_first(done)) {
+        if (hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) return FOCR_EHIP;
+        focr_dev_mark(done);
+      }
+    }
+    hipLaunchKernelGGL(kern, dim3((unsigned)tiles), dim3(64 * PGNW), LDS, st, a);
   }
+  if (p.thin_rows > 16) hipLaunchKernelGGL((paged_thin_kernel<T, D, 2>), dim3((unsigned)thin), dim3(256), 0, st, a);
+  else if (p.thin_rows) hipLaunchKernelGGL((paged_thin_kernel<T, D, 1>), dim3((unsigned)thin), dim3(256), 0, st, a);
+  if (need) hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3((unsigned)rows), dim3(256), 0, st, a);
   return FOCR_OK;
 }
 
@@ -737,8 +1044,8 @@ extern "C" int focr_paged_attention_fwd(const void* q, long ldt, long ldh, const
   const bool wo = pg_aligned(o) && (((ldto | ldho) * pg_esize(dtype)) & 15) == 0;
 #define PG_RUN(T, DD)                                                                                                       \
   rc = pg_run<T, DD>(PgArgs<T>{(const T*)q, ldt, ldh, (const T*)k_pages, (const T*)v_pages, c, (T*)o, ldto, ldho, (float*)ws, \
-                               nullptr, max_q, heads, kv_heads, heads / kv_heads, 1, 0, causal ? 1 : 0, 0, wq, wo,             \
-                               scale * 1.4426950408889634f}, ws_bytes, dim, (hipStream_t)stream)
+                               nullptr, max_q, heads, kv_heads, heads / kv_heads, 1, 0, 0, causal ? 1 : 0, 0, wq, wo,             \
+                               scale * 1.4426950408889634f}, ws_bytes, (hipStream_t)stream)
 #define PG_RUN_D(T)                    \
   if (dim == 64) PG_RUN(T, 64);        \
   else if (dim == 128) PG_RUN(T, 128); \
@@ -747,6 +1054,10 @@ extern "C" int focr_paged_attention_fwd(const void* q, long ldt, long ldh, const
   else if (dtype == FOCR_DT_BF16) { PG_RUN_D(bf16_t); }
   else { PG_RUN_D(f16_t); }
   FOCR_CHECK_ARG(rc != FOCR_EINVAL, "workspace missing or too small (focr_paged_attention_ws_bytes)");
+  if (rc == FOCR_EHIP) {
+    focr_set_error("%s: hipFuncSetAttribute failed", __func__);
+    return rc;
+  }
   if (rc == FOCR_EUNSUPPORTED) {
     focr_set_error("%s: too many sequences, heads and splits for one launch", __func__);
     return rc;
