@@ -227,10 +227,12 @@ __device__ __forceinline__ void pg_fill_nan(const PgArgs<T>& a, const PagedSeq& 
 // The next tile's loads go out between the two products.  MFMA time is a tenth of the bytes' (16-bit) to a third (fp32).
 // ======================================================================================================================
 #define PG_MAX_CHUNK 8192
-// queries that take 32 registers or more go through LDS: at most 256 registers keep two waves on a SIMD (one where the sums
-// of 32 rows x 256 alone take half of them)
+// Queries that take 32 registers or more go through LDS.  At most 256 registers keep two waves on a SIMD; 16-bit rows of 256
+// (106 us, spilling at two waves 132: 32 sequences of 4000 tokens, 4 key heads) and 32 rows x 256 take one
 template <typename T, int D, int NT> constexpr bool pg_thin_q_lds() { return NT * D * sizeof(T) >= 512; }
-template <typename T, int D, int NT> constexpr int pg_thin_waves() { return NT * D <= 64 ? 4 : NT * D <= 256 ? 2 : 1; }
+template <typename T, int D, int NT> constexpr int pg_thin_waves() {
+  return NT * D <= 64 ? 4 : D == 256 && (NT == 2 || sizeof(T) == 2) ? 1 : 2;
+}
 template <typename T, int D, int NT>
 __global__ __launch_bounds__(256, (pg_thin_waves<T, D, NT>())) void paged_thin_kernel(PgArgs<T> a) {
   constexpr int ES = sizeof(T), EC = 16 / ES;          // elements of a chunk
@@ -532,7 +534,7 @@ __global__ __launch_bounds__(256, (pg_thin_waves<T, D, NT>())) void paged_thin_k
 }
 
 // ======================================================================================================================
-// Many rows (a chunk's tokens x the heads that share a key head, flattened: a block takes 32 NQ NW neighbouring rows, so one
+// Many rows (a chunk's tokens x the heads that share a key head, flattened: a block takes 32 NW neighbouring rows, so one
 // staged tile of keys serves every head of the group): bound by the matrix instructions.  32 x 32 tiles in the same
 // orientation as above -- S^T = K Q^T leaves a lane one query column, whose weights are B of O^T = V^T P^T as they stand -- with
 // KT keys and values at a time in LDS, double-buffered by direct loads, 16-byte chunks XOR-swizzled by row so that both the
@@ -548,16 +550,16 @@ __device__ __forceinline__ uint2 pg_read_tr(const char* p) {
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pg_s16x4*)p));
 }
 
-template <typename T, int D, int NQ> constexpr int pg_tile_waves() { return NQ * D * sizeof(T) <= 512 ? 2 : 1; }
-template <typename T, int D, int NQ, int NW>
-__global__ __launch_bounds__(64 * NW, (pg_tile_waves<T, D, NQ>())) void paged_tile_kernel(PgArgs<T> a) {
+template <typename T, int D, int NW> constexpr int pg_tile_waves() { return NW == 8 || D * sizeof(T) <= 512 ? 2 : 1; }
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(64 * NW, (pg_tile_waves<T, D, NW>())) void paged_tile_kernel(PgArgs<T> a) {
   constexpr int ES = sizeof(T), EC = 16 / ES, ROWB = D * ES, CPR = ROWB / 16;
   constexpr int KT = ROWB <= 256 ? 64 : 32, NS = KT / 32;
   constexpr int NU = ROWB / 32;                        // contraction steps of S^T (pairs of chunks)
   constexpr int RPI = 64 / CPR;                        // rows one direct load of a wave brings
   constexpr int NL = KT / (RPI * NW);                  // such loads per wave, for K and for V
   constexpr int DT = D / 32, PT = ES == 4 ? 4 : 2;     // O^T tiles; contraction steps of O^T per 32 keys
-  constexpr int ROWS = 32 * NQ * NW;
+  constexpr int ROWS = 32 * NW;
   extern __shared__ __attribute__((aligned(128))) char pg_smem[];
   char* const ksm = pg_smem;                           // [2][KT][ROWB]
   char* const vsm = pg_smem + 2 * KT * ROWB;
@@ -596,23 +598,16 @@ __global__ __launch_bounds__(64 * NW, (pg_tile_waves<T, D, NQ>())) void paged_ti
   const int nt = k1 > k0 ? (k1 - k0 + KT - 1) / KT : 0;
 
   // this wave's rows: one query column per lane
-  u32x4 qf[NQ][NU];
-  int vis[NQ], wvmin = INT32_MAX, wvmax = 0;
+  u32x4 qf[NU];
+  const long row = r0 + wave * 32 + l32;
+  const bool ok = row < R;
+  const long tok = ok ? row / a.group : 0;
+  const int head = kh * a.group + (ok ? (int)(row - tok * a.group) : 0);
+  const int vis = ok ? paged_visible(sq.len, sq.n, (int)tok, a.causal) : 0;
+  int wvmin = ok ? vis : INT32_MAX, wvmax = vis;
+  const T* p = a.q + (sq.t0 + tok) * a.ldt + head * a.ldh + hh * EC;
 #pragma unroll
-  for (int t = 0; t < NQ; ++t) {
-    const long r = r0 + (wave * NQ + t) * 32 + l32;
-    const bool ok = r < R;
-    const long i = ok ? r / a.group : 0;
-    const int h = kh * a.group + (ok ? (int)(r - i * a.group) : 0);
-    vis[t] = ok ? paged_visible(sq.len, sq.n, (int)i, a.causal) : 0;
-    if (ok) {
-      wvmin = vis[t] < wvmin ? vis[t] : wvmin;
-      wvmax = vis[t] > wvmax ? vis[t] : wvmax;
-    }
-    const T* p = a.q + (sq.t0 + i) * a.ldt + h * a.ldh + hh * EC;
-#pragma unroll
-    for (int u = 0; u < NU; ++u) qf[t][u] = ok ? pg_load_chunk(p + u * 2 * EC, a.wide_q) : u32x4{0, 0, 0, 0};
-  }
+  for (int u = 0; u < NU; ++u) qf[u] = ok ? pg_load_chunk(p + u * 2 * EC, a.wide_q) : u32x4{0, 0, 0, 0};
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
     const int x = __shfl_xor(wvmin, o, 64), y = __shfl_xor(wvmax, o, 64);
@@ -640,7 +635,7 @@ __global__ __launch_bounds__(64 * NW, (pg_tile_waves<T, D, NQ>())) void paged_ti
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int row = (i * NW + wave) * RPI + lane / CPR;
-      const bool ok = pg[i] >= 0 && pg[i] < c.num_pages;
+      const bool ok = (uint32_t)pg[i] < (uint32_t)c.num_pages;
       bad_page |= !ok;
       const long at = (ok ? pg[i] : 0) * page_bytes + (long)(key_of(base, i) & slot_mask) * ROWB
                       + (((lane % CPR) ^ pg_swz<CPR>(row)) * 16);
@@ -651,21 +646,34 @@ __global__ __launch_bounds__(64 * NW, (pg_tile_waves<T, D, NQ>())) void paged_ti
                                        (__attribute__((address_space(3))) void*)(vsm + dst), 16, 0, 0);
     }
   };
+  // LDS offsets.  Rows enter the swizzle by their last four bits, of which a lane's row fixes all but constants of the unrolled
+  // loops: a few lane offsets, the rest are immediate (left to itself the compiler keeps every address and spills them)
+  constexpr bool LEAN = CPR > 16;                      // wide rows: one offset and an xor per read, the registers are short
+  constexpr int NKB = LEAN ? 1 : CPR == 8 ? 4 : 8;     // chunk pairs up to the width of the swizzle
+  constexpr int NVB = LEAN ? 1 : CPR == 8 ? 2 : 4;     // the same in O^T tiles (16-bit types)
+  int koff[NKB], voff[2][NVB];
+#pragma unroll
+  for (int j = 0; j < NKB; ++j) koff[j] = l32 * ROWB + (((2 * j + hh) ^ pg_swz<CPR>(l32)) << 4);
+  const int vrow = hh * 4 + (lane >> 2 & 3), vchunk = (lane >> 4 & 1) * 2 + (lane >> 1 & 1);
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+#pragma unroll
+    for (int j = 0; j < NVB; ++j)
+      voff[e][j] = (vrow + e * 8) * ROWB + (((4 * j + vchunk) ^ pg_swz<CPR>(vrow + e * 8)) << 4) + (lane & 1) * 8;
   // A operand of O^T: 32 values d of the keys sub * 32 + step * (32 / PT) ..
   auto v_frag = [&](const char* v, int sub, int step, int dt) {
     u32x4 r;
     if constexpr (ES == 4) {
+      const int lane_at = ((l32 >> 2) ^ (hh * 8)) << 4;            // swizzle of row 4 hh; the rest is one xor per word
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int row = sub * 32 + step * 8 + hh * 4 + e, d = dt * 32 + l32;
-        r[e] = *(const uint32_t*)(v + row * ROWB + (((d >> 2) ^ pg_swz<CPR>(row)) << 4) + (d & 3) * 4);
-      }
+      for (int e = 0; e < 4; ++e)
+        r[e] = *(const uint32_t*)(v + (lane_at ^ (((dt & 1) * 8) ^ (e * 2) ^ (step & 1)) << 4) + hh * 4 * ROWB + (l32 & 3) * 4
+                                  + (sub * 32 + step * 8 + e) * ROWB + (dt >> 1) * 256);
     } else {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int row = sub * 32 + step * 16 + e * 8 + hh * 4 + (lane >> 2 & 3);
-        const int col = (dt * 32 + (lane >> 4 & 1) * 16 + (lane & 3) * 4) * 2;
-        const uint2 x = pg_read_tr(v + row * ROWB + (((col >> 4) ^ pg_swz<CPR>(row)) << 4) + (col & 15));
+        const char* at = LEAN ? v + (voff[e][0] ^ (dt & 3) << 6) + dt / 4 * 256 : v + voff[e][dt % NVB] + dt / NVB * 256;
+        const uint2 x = pg_read_tr(at + (sub * 32 + step * 16) * ROWB);
         r[2 * e] = x.x;
         r[2 * e + 1] = x.y;
       }
@@ -673,15 +681,10 @@ __global__ __launch_bounds__(64 * NW, (pg_tile_waves<T, D, NQ>())) void paged_ti
     return r;
   };
 
-  f32x16 acc[NQ][DT];
-  float m[NQ], l[NQ];
+  f32x16 acc[DT];
+  float m = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int t = 0; t < NQ; ++t) {
-    m[t] = -INFINITY;
-    l[t] = 0.f;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) acc[t][dt] = f32x16{0};
-  }
+  for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x16{0};
   if (nt) {
     find_pages(k0);
     stage(k0, 0);
@@ -710,34 +713,32 @@ __global__ __launch_bounds__(64 * NW, (pg_tile_waves<T, D, NQ>())) void paged_ti
 #pragma unroll 1
         for (int sub = 0; sub < NS; ++sub)
 #pragma unroll 1
-          for (int step = 0; step < PT; ++step)
+          for (int step = 0; step < PT; ++step) {
+            u32x4 see;
 #pragma unroll
-            for (int t = 0; t < NQ; ++t) {
-              u32x4 see;
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                if constexpr (ES == 4) see[j] = base + sub * 32 + step * 8 + hh * 4 + j < vis[t] ? PgMma<T>::ONE : 0u;
-                else {
-                  const int key = base + sub * 32 + step * 16 + (j >> 1) * 8 + hh * 4 + (2 * j & 3);
-                  see[j] = (key < vis[t] ? PgMma<T>::ONE : 0u) | (key + 1 < vis[t] ? PgMma<T>::ONE << 16 : 0u);
-                }
-              }
-#pragma unroll
-              for (int dt = 0; dt < DT; ++dt) {
-                const u32x4 vf = v_frag(vt, sub, step, dt);
-                const f32x16 z = {0};
-                const f32x16 pos = PgMma<T>::mma32(pg_class<T, 1>(vf), see, z);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) acc[t][dt][i] = pg_with_nonfinite(acc[t][dt][i], pos[i], 0.f, 0.f);
-                const f32x16 neg = PgMma<T>::mma32(pg_class<T, 2>(vf), see, z);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) acc[t][dt][i] = pg_with_nonfinite(acc[t][dt][i], 0.f, neg[i], 0.f);
-                const f32x16 nan = PgMma<T>::mma32(pg_class<T, 3>(vf), see, z);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) acc[t][dt][i] = pg_with_nonfinite(acc[t][dt][i], 0.f, 0.f, nan[i]);
-                __builtin_amdgcn_sched_barrier(0);
+            for (int j = 0; j < 4; ++j) {
+              if constexpr (ES == 4) see[j] = base + sub * 32 + step * 8 + hh * 4 + j < vis ? PgMma<T>::ONE : 0u;
+              else {
+                const int key = base + sub * 32 + step * 16 + (j >> 1) * 8 + hh * 4 + (2 * j & 3);
+                see[j] = (key < vis ? PgMma<T>::ONE : 0u) | (key + 1 < vis ? PgMma<T>::ONE << 16 : 0u);
               }
             }
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+              const u32x4 vf = v_frag(vt, sub, step, dt);
+              const f32x16 z = {0};
+              const f32x16 pos = PgMma<T>::mma32(pg_class<T, 1>(vf), see, z);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) acc[dt][i] = pg_with_nonfinite(acc[dt][i], pos[i], 0.f, 0.f);
+              const f32x16 neg = PgMma<T>::mma32(pg_class<T, 2>(vf), see, z);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) acc[dt][i] = pg_with_nonfinite(acc[dt][i], 0.f, neg[i], 0.f);
+              const f32x16 nan = PgMma<T>::mma32(pg_class<T, 3>(vf), see, z);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) acc[dt][i] = pg_with_nonfinite(acc[dt][i], 0.f, 0.f, nan[i]);
+              __builtin_amdgcn_sched_barrier(0);
+            }
+          }
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < KT * ROWB / (1024 * NW); ++i) {
@@ -750,61 +751,54 @@ __global__ __launch_bounds__(64 * NW, (pg_tile_waves<T, D, NQ>())) void paged_ti
       }
     }
     if (base >= wvmax) continue;                       // nothing here for this wave's rows
-    f32x16 sc[NQ][NS];
+    f32x16 sc[NS];
 #pragma unroll
     for (int sub = 0; sub < NS; ++sub) {
-#pragma unroll
-      for (int t = 0; t < NQ; ++t) sc[t][sub] = f32x16{0};
-      const int row = sub * 32 + l32;
+      sc[sub] = f32x16{0};
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
-        const u32x4 kf = *(const u32x4*)(kt + row * ROWB + (((2 * u + hh) ^ pg_swz<CPR>(row)) << 4));
-#pragma unroll
-        for (int t = 0; t < NQ; ++t) sc[t][sub] = PgMma<T>::mma32(kf, qf[t][u], sc[t][sub]);
+        const char* at = LEAN ? kt + (koff[0] ^ (u & 7) << 5) + u / 8 * 256 : kt + koff[u % NKB] + u / NKB * 256;
+        const u32x4 kf = *(const u32x4*)(at + sub * 32 * ROWB);
+        sc[sub] = PgMma<T>::mma32(kf, qf[u], sc[sub]);
       }
     }
     if (base + KT > wvmin) {
 #pragma unroll
-      for (int t = 0; t < NQ; ++t)
-#pragma unroll
-        for (int sub = 0; sub < NS; ++sub)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (base + sub * 32 + 8 * (i >> 2) + 4 * hh + (i & 3) >= vis[t]) sc[t][sub][i] = -INFINITY;
-    }
-    u32x4 pf[NQ][NS][PT];
-#pragma unroll
-    for (int t = 0; t < NQ; ++t) {
-      float mx = m[t];
-#pragma unroll
       for (int sub = 0; sub < NS; ++sub)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[t][sub][i]);
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-      const float ref = mx == -INFINITY ? 0.f : mx * a.c2;
-      if (__any(mx > m[t])) {
-        const float al = __builtin_amdgcn_exp2f(m[t] * a.c2 - ref);
-        l[t] *= al;
+        for (int i = 0; i < 16; ++i)
+          if (base + sub * 32 + 8 * (i >> 2) + 4 * hh + (i & 3) >= vis) sc[sub][i] = -INFINITY;
+    }
+    u32x4 pf[NS][PT];
+    float mx = m;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) acc[t][dt] *= al;
-        m[t] = mx;
+    for (int sub = 0; sub < NS; ++sub)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[sub][i]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    const float ref = mx == -INFINITY ? 0.f : mx * a.c2;
+    if (__any(mx > m)) {
+      const float al = __builtin_amdgcn_exp2f(m * a.c2 - ref);
+      l *= al;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) acc[dt] *= al;
+      m = mx;
+    }
+#pragma unroll
+    for (int sub = 0; sub < NS; ++sub) {
+      float p[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(fmaf(sc[sub][i], a.c2, -ref));
+        l += p[i];
       }
 #pragma unroll
-      for (int sub = 0; sub < NS; ++sub) {
-        float p[16];
+      for (int step = 0; step < PT; ++step)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          p[i] = __builtin_amdgcn_exp2f(fmaf(sc[t][sub][i], a.c2, -ref));
-          l[t] += p[i];
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (ES == 4) pf[sub][step][j] = __float_as_uint(p[step * 4 + j]);
+          else pf[sub][step][j] = pg_pack<T>(p[step * 8 + 2 * j], p[step * 8 + 2 * j + 1]);
         }
-#pragma unroll
-        for (int step = 0; step < PT; ++step)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if constexpr (ES == 4) pf[t][sub][step][j] = __float_as_uint(p[step * 4 + j]);
-            else pf[t][sub][step][j] = pg_pack<T>(p[step * 8 + 2 * j], p[step * 8 + 2 * j + 1]);
-          }
-      }
     }
 #pragma unroll
     for (int sub = 0; sub < NS; ++sub)
@@ -813,82 +807,80 @@ __global__ __launch_bounds__(64 * NW, (pg_tile_waves<T, D, NQ>())) void paged_ti
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
           const u32x4 vf = v_frag(vt, sub, step, dt);
-#pragma unroll
-          for (int t = 0; t < NQ; ++t) acc[t][dt] = PgMma<T>::mma32(vf, pf[t][sub][step], acc[t][dt]);
+          acc[dt] = PgMma<T>::mma32(vf, pf[sub][step], acc[dt]);
         }
   }
   const bool any_bad = __syncthreads_or(bad_page);
 
   // out: lane = row, four neighbouring values d = 32 dt + 8 q + 4 (l / 32) + ..
+  float ls = l + __shfl_xor(l, 32, 64);
+  if (any_bad) ls = NAN;
+  if (!ok) return;
+  const float inv = direct ? (ls == 0.f ? 0.f : 1.f / ls) : 1.f;
+  T* o = a.o + (sq.t0 + tok) * a.ldto + head * a.ldho + 4 * hh;
+  const long out_row = ((long)split * c.tokens + sq.t0 + tok) * a.heads + head;
 #pragma unroll
-  for (int t = 0; t < NQ; ++t) {
-    const long r = r0 + (wave * NQ + t) * 32 + l32;
-    float ls = l[t] + __shfl_xor(l[t], 32, 64);
-    if (any_bad) ls = NAN;
-    if (r >= R) continue;
-    const long i = r / a.group;
-    const int h = kh * a.group + (int)(r - i * a.group);
-    const float inv = direct ? (ls == 0.f ? 0.f : 1.f / ls) : 1.f;
-    T* o = a.o + (sq.t0 + i) * a.ldto + h * a.ldho + 4 * hh;
-    const long row = ((long)split * c.tokens + sq.t0 + i) * a.heads + h;
+  for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+    for (int q = 0; q < 4; ++q) {
+      float v[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = ls == 0.f ? 0.f : acc[t][dt][4 * q + e] * inv;
-        if (direct) pg_store_row<T, 4>(o + dt * 32 + q * 8, v, a.wide_o);
-        else *(f32x4*)(a.part + row * D + dt * 32 + q * 8 + 4 * hh) = f32x4{v[0], v[1], v[2], v[3]};
-      }
-    if (!direct && hh == 0) a.ml[row] = float2{any_bad ? 0.f : m[t] * a.c2, ls};
-  }
+      for (int e = 0; e < 4; ++e) v[e] = ls == 0.f ? 0.f : acc[dt][4 * q + e] * inv;
+      if (direct) pg_store_row<T, 4>(o + dt * 32 + q * 8, v, a.wide_o);
+      else *(f32x4*)(a.part + out_row * D + dt * 32 + q * 8 + 4 * hh) = f32x4{v[0], v[1], v[2], v[3]};
+    }
+  if (!direct && hh == 0) a.ml[out_row] = float2{any_bad ? 0.f : m * a.c2, ls};
 }
 
-// ---- joins the splits of a row: one block per (token, head), the splits dealt out to its 4 waves ------------------------
-template <typename T, int D>
+// ---- joins the splits of a row.  WPR waves of a block of 4 share a (token, head): 1 where rows are many and splits few, 4 where
+// a long cache was cut into dozens (69 000 rows, 4 splits: 51 us with a block each, most of it for starting blocks) ----------
+template <typename T, int D, int WPR>
 __global__ __launch_bounds__(256) void paged_join_kernel(PgArgs<T> a) {
   constexpr int E = D / 64;
   __shared__ float wmax[4], wsum[4], acc[3][D];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long row = blockIdx.x, t = row / a.heads;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = wave % WPR;
+  const long row = (long)blockIdx.x * (4 / WPR) + wave / WPR, rows = a.c.tokens * a.heads;
+  if (row >= rows) return;                             // (with 4 waves a row there is no such row)
+  const long t = row / a.heads;
   const int h = (int)(row - t * a.heads), s = pg_seq_of_row(a.c, t, lane);
   const PagedSeq sq = paged_seq(a.c, s);
   const long i = t - sq.t0;
   const int chunk = (long)sq.n * a.group <= a.thin_rows ? a.chunk : a.tile_chunk;
   if (i < 0 || i >= sq.n || sq.bad || sq.n > a.max_q || sq.len <= chunk) return;
   const int n = (paged_visible(sq.len, sq.n, (int)i, a.causal) + chunk - 1) / chunk;
-  const long step = a.c.tokens * a.heads;
   float mx = -INFINITY;
-  for (int k = threadIdx.x; k < n; k += 256) mx = fmaxf(mx, a.ml[row + k * step].x);
+  for (int k = part * 64 + lane; k < n; k += 64 * WPR) mx = fmaxf(mx, a.ml[row + k * rows].x);
   mx = wave_max(mx);
-  if (lane == 0) wmax[wave] = mx;
-  __syncthreads();
-  mx = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
+  if constexpr (WPR == 4) {
+    if (lane == 0) wmax[wave] = mx;
+    __syncthreads();
+    mx = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
+  }
   float ls = 0.f, v[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) v[e] = 0.f;
 #pragma unroll 4
-  for (int k = wave; k < n; k += 4) {
-    const float2 ml = a.ml[row + k * step];
+  for (int k = part; k < n; k += WPR) {
+    const float2 ml = a.ml[row + k * rows];
     const float w = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mx);
     ls += pg_share(ml.y, ml.x - mx);
-    const float* p = a.part + (row + k * step) * D + lane * E;
+    const float* p = a.part + (row + k * rows) * D + lane * E;
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] += w * p[e];
   }
-  if (lane == 0) wsum[wave] = ls;
-  if (wave)
-    for (int e = 0; e < E; ++e) acc[wave - 1][lane * E + e] = v[e];
-  __syncthreads();
-  if (wave) return;
-  ls = wsum[0] + wsum[1] + wsum[2] + wsum[3];
+  if constexpr (WPR == 4) {
+    if (lane == 0) wsum[wave] = ls;
+    if (wave)
+      for (int e = 0; e < E; ++e) acc[wave - 1][lane * E + e] = v[e];
+    __syncthreads();
+    if (wave) return;
+    ls = wsum[0] + wsum[1] + wsum[2] + wsum[3];
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] += acc[0][lane * E + e] + acc[1][lane * E + e] + acc[2][lane * E + e];
+  }
   T* o = a.o + t * a.ldto + h * a.ldho + lane * E;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const float x = v[e] + acc[0][lane * E + e] + acc[1][lane * E + e] + acc[2][lane * E + e];
-    o[e] = (T)(ls == 0.f ? 0.f : x / ls);
-  }
+  for (int e = 0; e < E; ++e) o[e] = (T)(ls == 0.f ? 0.f : v[e] / ls);
 }
 
 // ---- C entries ---------------------------------------------------------------------------------------------------------
@@ -934,21 +926,24 @@ extern "C" int focr_paged_append(const void* k_new, const void* v_new, long ldtk
 // of very different lengths still fill the card evenly (64 sequences of 100 .. 8190 tokens x 8 heads, bf16, 128 wide: 2048
 // blocks 198 us, 4096 193 us, 8192 200 us), but no fewer than 1024 keys in a block while there are blocks enough for two on each
 // CU: a block's start and end cost as much as some hundred keys (2 sequences of 131k: 1024 keys 205 us, 512 224 us, 256 254 us).
+//
+// Calls with longer chunks go to the tile kernel: 128 rows a block, and split over keys only when there are fewer than two such
+// blocks a CU (24 chunks of 1 .. 764 tokens x 32 heads, bf16: 221 us unsplit, 232 / 240 us cut for 1024 / 2048 blocks: the parts
+// are written and read in fp32).  256 rows a block halve the reads from LDS per product, but make one block a CU: taken when
+// 128-row blocks would fill the card twice over and sequences are long (4096 tokens after 12288: 1058 -> 948 us; the 24 chunks:
+// 221 -> 250 us).  In a ragged call that has mostly short sequences those go to the thin kernel in a launch of their own; with
+// 32 rows a sequence or more on average the tiles take them along (the 24 chunks, 11 of them single tokens: 303 -> 221 us).
 struct PgPlan {
   int thin_rows;           // sequences of at most this many rows go to the thin kernel, the rest to the tiles
   int nsplit, chunk;       // of the thin kernel
   int tsplit, tile_chunk;  // of the tiles
+  int tile_waves;          // 32 rows each
 };
-#ifndef PGNQ
-#define PGNQ 1
-#define PGNW 4
-#endif
-template <typename T, int D> constexpr int pg_tile_rows() { return 32 * PGNQ * PGNW; }
 static PgPlan pg_plan(long tokens, int seqs, int kv_heads, int group, int max_q, int max_kv, bool ragged) {
-  PgPlan p = {0, 1, 128, 1, INT32_MAX};
+  PgPlan p = {0, 1, 128, 1, INT32_MAX, 4};
   const long rmax = (long)max_q * group;
   if (rmax <= 32) p.thin_rows = rmax <= 16 ? 16 : 32;
-  else if (ragged) p.thin_rows = group <= 16 ? 16 : group <= 32 ? 32 : 0;
+  else if (ragged && tokens * group <= 32l * seqs) p.thin_rows = group <= 16 ? 16 : group <= 32 ? 32 : 0;
   if (p.thin_rows) {
     const long groups = (long)seqs * kv_heads, want = (4096 + groups - 1) / groups;
     long chunk = (max_kv + want - 1) / want;
@@ -971,6 +966,7 @@ static PgPlan pg_plan(long tokens, int seqs, int kv_heads, int group, int max_q,
       p.tsplit = (int)((max_kv + chunk - 1) / chunk);
       p.tile_chunk = (int)chunk;
     }
+    if (blocks >= 1024 && tokens * group >= 1024l * seqs) p.tile_waves = 8;
   }
   return p;
 }
@@ -990,10 +986,27 @@ extern "C" long focr_paged_attention_ws_bytes(long tokens, int seqs, int heads, 
   return a > b ? a : b;
 }
 
+template <typename T, int D, int NW>
+static int pg_launch_tiles(const PgArgs<T>& a, long blocks, hipStream_t st) {
+  constexpr int LDS = 4 * (D * sizeof(T) <= 256 ? 64 : 32) * D * sizeof(T);
+  auto kern = paged_tile_kernel<T, D, NW>;
+  if (LDS > 49152) {
+    static focr_dev_flags done;
+    if (focr_dev_first(done)) {
+      if (hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) return FOCR_EHIP;
+      focr_dev_mark(done);
+    }
+  }
+  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(64 * NW), LDS, st, a);
+  return FOCR_OK;
+}
+
 template <typename T, int D>
 static int pg_run(PgArgs<T> a, long ws_bytes, hipStream_t st) {
   const PagedShape& c = a.c;
-  const PgPlan p = pg_plan(c.tokens, c.seqs, a.kv_heads, a.group, a.max_q, c.max_kv, c.q_start != nullptr);
+  PgPlan p = pg_plan(c.tokens, c.seqs, a.kv_heads, a.group, a.max_q, c.max_kv, c.q_start != nullptr);
+  constexpr bool WIDE = D * sizeof(T) <= 512;          // fp32 x 256: a wave's queries and sums need the registers of two
+  if (!WIDE) p.tile_waves = 4;
   a.nsplit = p.nsplit;
   a.chunk = p.chunk;
   a.tile_chunk = p.tile_chunk;
@@ -1003,25 +1016,21 @@ static int pg_run(PgArgs<T> a, long ws_bytes, hipStream_t st) {
     if (!a.part || ws_bytes < need) return FOCR_EINVAL;
     a.ml = (float2*)(a.part + need / ((D + 2) * 4) * D);
   }
-  const long rmax = (long)a.max_q * a.group;
   const long thin = (long)p.nsplit * a.kv_heads * c.seqs;
-  const long tiles = paged_tiles(c.tokens, c.seqs, a.group, pg_tile_rows<T, D>()) * a.kv_heads * p.tsplit;
+  const long tiles = paged_tiles(c.tokens, c.seqs, a.group, 32 * p.tile_waves) * a.kv_heads * p.tsplit;
   if (thin > INT32_MAX || tiles > INT32_MAX || rows > INT32_MAX) return FOCR_EUNSUPPORTED;
-  if (rmax > 32) {
-    constexpr int LDS = 4 * (D * sizeof(T) <= 256 ? 64 : 32) * D * sizeof(T);
-    auto kern = paged_tile_kernel<T, D, PGNQ, PGNW>;
-    if (LDS > 49152) {
-      static focr_dev_flags done;
-      if (focr_dev_first(done)) {
-        if (hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) return FOCR_EHIP;
-        focr_dev_mark(done);
-      }
-    }
-    hipLaunchKernelGGL(kern, dim3((unsigned)tiles), dim3(64 * PGNW), LDS, st, a);
+  if ((long)a.max_q * a.group > 32) {
+    int rc;
+    if constexpr (WIDE) rc = p.tile_waves == 8 ? pg_launch_tiles<T, D, 8>(a, tiles, st) : pg_launch_tiles<T, D, 4>(a, tiles, st);
+    else rc = pg_launch_tiles<T, D, 4>(a, tiles, st);
+    if (rc) return rc;
   }
   if (p.thin_rows > 16) hipLaunchKernelGGL((paged_thin_kernel<T, D, 2>), dim3((unsigned)thin), dim3(256), 0, st, a);
   else if (p.thin_rows) hipLaunchKernelGGL((paged_thin_kernel<T, D, 1>), dim3((unsigned)thin), dim3(256), 0, st, a);
-  if (need) hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3((unsigned)rows), dim3(256), 0, st, a);
+  if (need) {
+    if (p.nsplit > 16 || p.tsplit > 16) hipLaunchKernelGGL((paged_join_kernel<T, D, 4>), dim3((unsigned)rows), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((paged_join_kernel<T, D, 1>), dim3(cdiv(rows, 4)), dim3(256), 0, st, a);
+  }
   return FOCR_OK;
 }
 

@@ -27,17 +27,18 @@ from . import _lib
 from .kernels import _RAW_STREAM
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_PAGES, _DIMS = frozenset(8 << i for i in range(8)), (64, 128, 256)
+_EVEN = "without q_start every sequence has the same number of rows; %d tokens, %d sequences"
 
 
-def _need(ok, what):
+def _need(ok, what, *args):
     if not ok:
-        raise RuntimeError("fudanocr_amd.decode: " + what)
+        raise RuntimeError("fudanocr_amd.decode: " + (what % args if args else what))
 
 
 def _launch(device, name, *args):
-    """the entry point on the current stream of the tensors' device, whatever device is current"""
-    _need(device.type == "cuda", "tensors must be on the GPU, got %s" % device)
-    if device.index == torch.cuda.current_device():
+    """the entry point on the current stream of the tensors' device (an index), whatever device is current"""
+    if device == torch.cuda.current_device():
         _lib.call(name, *args, _stream(device))
     else:
         with torch.cuda.device(device):
@@ -45,61 +46,66 @@ def _launch(device, name, *args):
 
 
 def _stream(device):
-    return _RAW_STREAM(device.index) if _RAW_STREAM is not None else torch.cuda.current_stream(device).cuda_stream
+    return _RAW_STREAM(device) if _RAW_STREAM is not None else torch.cuda.current_stream(device).cuda_stream
 
 
-def _int32(t, shape, device, what):
-    _need(isinstance(t, torch.Tensor) and t.dtype == torch.int32 and tuple(t.shape) == tuple(shape) and t.is_contiguous()
-          and t.device == device, "%s must be a contiguous int32 tensor %s on %s" % (what, list(shape), device))
+def _on_gpu(t):
+    """the tensors' device as an index (`get_device` -- a device object per check costs more than the rest of it)"""
+    dev = t.get_device()
+    _need(dev >= 0, "tensors must be on the GPU, got %s", t.device)
+    return dev
+
+
+def _int32(t, shape, dev, what):
+    _need(t.dtype is torch.int32 and t.shape == shape and t.is_contiguous() and t.get_device() == dev,
+          "%s must be a contiguous int32 tensor %s on the same device as the others", what, tuple(shape))
 
 
 def _cache(k_pages, v_pages, table, kv_lens, q_start):
-    _need(k_pages.dim() == 4 and k_pages.shape == v_pages.shape and k_pages.dtype == v_pages.dtype
-          and k_pages.dtype in _DTYPES, "k_pages and v_pages must be two [num_pages, heads, page, dim] tensors of one type "
-          "(fp32, bf16 or fp16)")
-    _need(k_pages.is_contiguous() and v_pages.is_contiguous() and k_pages.device == v_pages.device,
+    shape, dt, dev = k_pages.shape, k_pages.dtype, k_pages.get_device()
+    _need(len(shape) == 4 and shape == v_pages.shape and dt is v_pages.dtype and dt in _DTYPES,
+          "k_pages and v_pages must be two [num_pages, heads, page, dim] tensors of one type (fp32, bf16 or fp16)")
+    _need(k_pages.is_contiguous() and v_pages.is_contiguous() and v_pages.get_device() == dev,
           "k_pages and v_pages must be contiguous and on one device")
-    num_pages, heads, page, dim = k_pages.shape
-    _need(8 <= page <= 1024 and page & (page - 1) == 0, "page must be a power of two from 8 to 1024, got %d" % page)
-    _need(dim in (64, 128, 256), "head dim must be 64, 128 or 256, got %d" % dim)
+    num_pages, heads, page, dim = shape
+    _need(page in _PAGES, "page must be a power of two from 8 to 1024, got %d", page)
+    _need(dim in _DIMS, "head dim must be 64, 128 or 256, got %d", dim)
     _need(num_pages > 0 and heads > 0, "the cache has no pages or no heads")
-    dev = k_pages.device
-    _need(isinstance(table, torch.Tensor) and table.dim() == 2 and table.shape[1] > 0, "table must be [seqs, pages per sequence]")
-    seqs = table.shape[0]
-    _int32(table, table.shape, dev, "table")
+    tshape = table.shape
+    _need(len(tshape) == 2 and tshape[1] > 0, "table must be [seqs, pages per sequence]")
+    seqs = tshape[0]
+    _int32(table, tshape, dev, "table")
     _int32(kv_lens, (seqs,), dev, "kv_lens")
     if q_start is not None:
         _int32(q_start, (seqs + 1,), dev, "q_start")
-    return num_pages, heads, page, dim, seqs
+    return num_pages, heads, page, dim, seqs, tshape[1], dt, dev
 
 
-def _rows(t, heads, dim, like, what):
-    _need(t.dim() == 3 and t.shape[2] == dim and (heads is None or t.shape[1] == heads) and t.dtype == like.dtype
-          and t.device == like.device, "%s must be [tokens, %s, %d] %s on %s"
-          % (what, "heads" if heads is None else heads, dim, like.dtype, like.device))
-    _need(t.stride(2) == 1 or t.numel() == 0, "%s must have contiguous rows of dim" % what)
-
-
-def _even(tokens, seqs, q_start):
-    _need(q_start is not None or seqs == 0 or tokens % seqs == 0,
-          "without q_start every sequence has the same number of rows; %d tokens, %d sequences" % (tokens, seqs))
+def _rows(t, heads, dim, dt, dev, what):
+    """-> the strides of the token and head axes"""
+    shape = t.shape
+    _need(len(shape) == 3 and shape[2] == dim and (heads is None or shape[1] == heads) and t.dtype is dt
+          and t.get_device() == dev, "%s must be [tokens, %s, %d] %s on the cache's device", what,
+          "heads" if heads is None else heads, dim, dt)
+    st = t.stride()
+    _need(st[2] == 1 or t.numel() == 0, "%s must have contiguous rows of dim", what)
+    return st[0], st[1]
 
 
 def paged_append(k_new, v_new, k_pages, v_pages, table, kv_lens, q_start=None):
     """writes the new tokens' keys and values [tokens, heads, dim] to their pages (positions kv_lens - n .. kv_lens - 1 of each
     sequence).  A token whose page the table does not name is dropped."""
-    num_pages, heads, page, dim, seqs = _cache(k_pages, v_pages, table, kv_lens, q_start)
-    _rows(k_new, heads, dim, k_pages, "k_new")
-    _rows(v_new, heads, dim, k_pages, "v_new")
+    num_pages, heads, page, dim, seqs, ld, dt, dev = _cache(k_pages, v_pages, table, kv_lens, q_start)
+    ks, vs = _rows(k_new, heads, dim, dt, dev, "k_new"), _rows(v_new, heads, dim, dt, dev, "v_new")
     tokens = k_new.shape[0]
     _need(v_new.shape[0] == tokens, "k_new and v_new must have the same tokens")
-    _even(tokens, seqs, q_start)
+    _need(q_start is not None or seqs == 0 or tokens % seqs == 0, _EVEN, tokens, seqs)
+    _on_gpu(k_pages)
     if tokens == 0 or seqs == 0:
         return
-    _launch(k_pages.device, "focr_paged_append", k_new.data_ptr(), v_new.data_ptr(), k_new.stride(0), k_new.stride(1),
-            v_new.stride(0), v_new.stride(1), k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), kv_lens.data_ptr(),
-            None if q_start is None else q_start.data_ptr(), tokens, seqs, heads, dim, page, table.shape[1], num_pages,
-            _DTYPES[k_pages.dtype])
+    _launch(dev, "focr_paged_append", k_new.data_ptr(), v_new.data_ptr(), ks[0], ks[1], vs[0], vs[1], k_pages.data_ptr(),
+            v_pages.data_ptr(), table.data_ptr(), kv_lens.data_ptr(), None if q_start is None else q_start.data_ptr(), tokens,
+            seqs, heads, dim, page, ld, num_pages, _DTYPES[dt])
 
 
 def paged_attention(q, k_pages, v_pages, table, kv_lens, q_start=None, causal=True, scale=None, max_q=None, max_kv=None,
@@ -110,36 +116,37 @@ def paged_attention(q, k_pages, v_pages, table, kv_lens, q_start=None, causal=Tr
     sees the positions 0 .. p, else all kv_lens of them; a token that sees nothing gets zeros.  scale: 1 / sqrt(dim) unless
     given, positive.  max_q / max_kv: bounds on a sequence's new tokens and on kv_lens that the caller knows (they size the
     launch; the defaults are the most the tensors allow).  out: where to write (not q's memory)."""
-    num_pages, kv_heads, page, dim, seqs = _cache(k_pages, v_pages, table, kv_lens, q_start)
-    _rows(q, None, dim, k_pages, "q")
+    num_pages, kv_heads, page, dim, seqs, ld, dt, dev = _cache(k_pages, v_pages, table, kv_lens, q_start)
+    qs = _rows(q, None, dim, dt, dev, "q")
     tokens, heads = q.shape[0], q.shape[1]
-    _need(heads > 0 and heads % kv_heads == 0, "%d heads over a cache of %d" % (heads, kv_heads))
-    _even(tokens, seqs, q_start)
-    scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
-    _need(0.0 < scale < math.inf, "scale must be positive and finite, got %r" % scale)
-    limit = table.shape[1] * page
+    _need(heads > 0 and heads % kv_heads == 0, "%d heads over a cache of %d", heads, kv_heads)
+    _need(q_start is not None or seqs == 0 or tokens % seqs == 0, _EVEN, tokens, seqs)
+    scale = dim ** -0.5 if scale is None else float(scale)
+    _need(0.0 < scale < math.inf, "scale must be positive and finite, got %r", scale)
+    limit = ld * page
     max_kv = limit if max_kv is None else min(int(max_kv), limit)
     if q_start is None:
         max_q = tokens // seqs if seqs else 0
     else:
         max_q = tokens if max_q is None else min(int(max_q), tokens)
     _need(max_q >= 0 and 0 <= max_kv < 2 ** 31, "max_q / max_kv out of range")
-    if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
-    else:
-        _rows(out, heads, dim, k_pages, "out")
+    if out is not None:
+        os = _rows(out, heads, dim, dt, dev, "out")
         _need(out.shape[0] == tokens, "out must have q's shape")
         _need(not _overlap(out, q), "out must not share q's memory")
+    _on_gpu(k_pages)
+    if out is None:
+        out, os = torch.empty((tokens, heads, dim), dtype=dt, device=q.device), (heads * dim, dim)
     if tokens == 0 or seqs == 0:
         return out
-    dt, dev = _DTYPES[q.dtype], q.device
-    n_ws = _lib.load().focr_paged_attention_ws_bytes(tokens, seqs, heads, kv_heads, dim, max_q, max_kv, dt)
+    code = _DTYPES[dt]
+    n_ws = _lib.load().focr_paged_attention_ws_bytes(tokens, seqs, heads, kv_heads, dim, max_q, max_kv, code)
     _need(n_ws >= 0, "arguments out of range")
-    ws = torch.empty(n_ws, dtype=torch.uint8, device=dev) if n_ws else None
-    _launch(dev, "focr_paged_attention_fwd", q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(), v_pages.data_ptr(),
-            table.data_ptr(), kv_lens.data_ptr(), None if q_start is None else q_start.data_ptr(), out.data_ptr(),
-            out.stride(0), out.stride(1), None if ws is None else ws.data_ptr(), n_ws, tokens, seqs, heads, kv_heads, dim, page,
-            table.shape[1], num_pages, max_q, max_kv, scale, int(bool(causal)), dt)
+    ws = torch.empty(n_ws, dtype=torch.uint8, device=q.device) if n_ws else None
+    _launch(dev, "focr_paged_attention_fwd", q.data_ptr(), qs[0], qs[1], k_pages.data_ptr(), v_pages.data_ptr(),
+            table.data_ptr(), kv_lens.data_ptr(), None if q_start is None else q_start.data_ptr(), out.data_ptr(), os[0], os[1],
+            None if ws is None else ws.data_ptr(), n_ws, tokens, seqs, heads, kv_heads, dim, page, ld, num_pages, max_q, max_kv,
+            scale, 1 if causal else 0, code)
     return out
 
 
@@ -161,32 +168,35 @@ def beam_select(logits, scores, finished=None, eos=None, n=None):
     Equal scores go to the lowest (beam, token).  NaN logits and beams whose score or normaliser is not finite rank as -inf.
 
     -> (scores fp32 [batch, n], parents int32 [batch, n], tokens int64 [batch, n], finished bool [batch, n])"""
-    _need(logits.dim() == 3 and logits.dtype in _DTYPES, "logits must be [batch, beams, vocab] in fp32, bf16 or fp16")
-    batch, beams, vocab = logits.shape
-    dev = logits.device
+    shape, dt, dev = logits.shape, logits.dtype, logits.get_device()
+    _need(len(shape) == 3 and dt in _DTYPES, "logits must be [batch, beams, vocab] in fp32, bf16 or fp16")
+    batch, beams, vocab = shape
     n = beams if n is None else int(n)
     _need(1 <= beams <= 64 and 1 <= n <= 64 and vocab >= 1 and n <= beams * vocab,
-          "beams and n must be 1 to 64 and n at most beams * vocab; got %d beams, n = %d, vocab %d" % (beams, n, vocab))
-    _need(logits.stride(2) == 1 or vocab == 1 or logits.numel() == 0, "logits must have contiguous rows of vocab")
-    _need(scores.dtype == torch.float32 and tuple(scores.shape) == (batch, beams) and scores.is_contiguous()
-          and scores.device == dev, "scores must be a contiguous fp32 tensor %s on %s" % ([batch, beams], dev))
+          "beams and n must be 1 to 64 and n at most beams * vocab; got %d beams, n = %d, vocab %d", beams, n, vocab)
+    ls = logits.stride()
+    _need(ls[2] == 1 or vocab == 1 or logits.numel() == 0, "logits must have contiguous rows of vocab")
+    _need(scores.dtype is torch.float32 and scores.shape == (batch, beams) and scores.is_contiguous()
+          and scores.get_device() == dev, "scores must be a contiguous fp32 tensor [batch, beams] on the logits' device")
     if finished is not None:
-        _need(finished.dtype == torch.bool and tuple(finished.shape) == (batch, beams) and finished.is_contiguous()
-              and finished.device == dev, "finished must be a contiguous bool tensor %s on %s" % ([batch, beams], dev))
+        _need(finished.dtype is torch.bool and finished.shape == (batch, beams) and finished.is_contiguous()
+              and finished.get_device() == dev, "finished must be a contiguous bool tensor [batch, beams] on the logits' device")
         _need(eos is not None, "finished beams need an eos")
     _need(eos is None or 0 <= int(eos) < vocab, "eos must be inside the vocabulary")
     eos = -1 if eos is None else int(eos)
-    out = (torch.empty((batch, n), dtype=torch.float32, device=dev), torch.empty((batch, n), dtype=torch.int32, device=dev),
-           torch.empty((batch, n), dtype=torch.int64, device=dev), torch.empty((batch, n), dtype=torch.bool, device=dev))
-    if batch == 0:
-        return out
-    dt = _DTYPES[logits.dtype]
-    n_ws = _lib.load().focr_beam_select_ws_bytes(batch, beams, vocab, n, dt)
-    ws = torch.empty(n_ws, dtype=torch.uint8, device=dev) if n_ws else None
-    _launch(dev, "focr_beam_select", logits.data_ptr(), logits.stride(0), logits.stride(1), scores.data_ptr(),
-            None if finished is None else finished.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(),
-            out[3].data_ptr(), None if ws is None else ws.data_ptr(), n_ws, batch, beams, vocab, n, eos, dt)
-    return out
+    _on_gpu(logits)
+    device = logits.device
+    out_scores, out_parents = (torch.empty((batch, n), dtype=t, device=device) for t in (torch.float32, torch.int32))
+    out_tokens, out_finished = (torch.empty((batch, n), dtype=t, device=device) for t in (torch.int64, torch.bool))
+    if batch:
+        code = _DTYPES[dt]
+        n_ws = _lib.load().focr_beam_select_ws_bytes(batch, beams, vocab, n, code)
+        ws = torch.empty(n_ws, dtype=torch.uint8, device=device) if n_ws else None
+        _launch(dev, "focr_beam_select", logits.data_ptr(), ls[0], ls[1], scores.data_ptr(),
+                None if finished is None else finished.data_ptr(), out_scores.data_ptr(), out_parents.data_ptr(),
+                out_tokens.data_ptr(), out_finished.data_ptr(), None if ws is None else ws.data_ptr(), n_ws, batch, beams, vocab,
+                n, eos, code)
+    return out_scores, out_parents, out_tokens, out_finished
 
 
 def beam_reorder(parents, table, kv_lens, spare, pages, table_out=None, spare_out=None):
@@ -198,34 +208,38 @@ def beam_reorder(parents, table, kv_lens, spare, pages, table_out=None, spare_ou
     layer) that the table stands for.  Before the call, the pages in `spare` and each beam's entries from its partial page on
     must be its own alone (`PagedCache` sees to that).  table_out / spare_out may be the inputs; a parent outside
     the group counts as the beam itself."""
-    _need(isinstance(parents, torch.Tensor) and parents.dim() == 2, "parents must be [groups, beams]")
-    groups, beams = parents.shape
-    dev, slots = parents.device, groups * beams
-    _int32(parents, parents.shape, dev, "parents")
+    pshape, dev = parents.shape, parents.get_device()
+    _need(len(pshape) == 2, "parents must be [groups, beams]")
+    groups, beams = pshape
+    slots = groups * beams
+    _int32(parents, pshape, dev, "parents")
     _need(1 <= beams <= 64 and slots <= 65535, "beams must be 1 to 64 and groups * beams at most 65535")
-    _need(table.dim() == 2 and table.shape[0] == slots and table.shape[1] > 0, "table must be [groups * beams, pages per sequence]")
-    _int32(table, table.shape, dev, "table")
+    tshape = table.shape
+    _need(len(tshape) == 2 and tshape[0] == slots and tshape[1] > 0, "table must be [groups * beams, pages per sequence]")
+    _int32(table, tshape, dev, "table")
     _int32(kv_lens, (slots,), dev, "kv_lens")
     _int32(spare, (slots,), dev, "spare")
     pages = list(pages)
     _need(len(pages) > 0, "no page tensors")
+    shape, dt = pages[0].shape, pages[0].dtype
     for p in pages:
-        _need(p.dim() == 4 and p.shape == pages[0].shape and p.dtype == pages[0].dtype and p.dtype in _DTYPES
-              and p.is_contiguous() and p.device == dev, "pages must be contiguous [num_pages, heads, page, dim] tensors of one "
-              "shape and type (fp32, bf16 or fp16) on %s" % dev)
-    num_pages, heads, page, dim = pages[0].shape
-    _need(8 <= page <= 1024 and page & (page - 1) == 0, "page must be a power of two from 8 to 1024, got %d" % page)
+        _need(len(shape) == 4 and p.shape == shape and p.dtype is dt and dt in _DTYPES and p.is_contiguous()
+              and p.get_device() == dev, "pages must be contiguous [num_pages, heads, page, dim] tensors of one shape and type "
+              "(fp32, bf16 or fp16) on the parents' device")
+    num_pages, heads, page, dim = shape
+    _need(page in _PAGES, "page must be a power of two from 8 to 1024, got %d", page)
     _need(num_pages > 0 and heads > 0 and dim > 0 and dim * pages[0].element_size() % 16 == 0,
           "rows of dim must be whole 16-byte units")
     table_out = torch.empty_like(table) if table_out is None else table_out
     spare_out = torch.empty_like(spare) if spare_out is None else spare_out
-    _int32(table_out, table.shape, dev, "table_out")
-    _int32(spare_out, spare.shape, dev, "spare_out")
+    _int32(table_out, tshape, dev, "table_out")
+    _int32(spare_out, (slots,), dev, "spare_out")
+    _on_gpu(parents)
     if slots:
         ptrs = (ctypes.c_void_p * len(pages))(*[p.data_ptr() for p in pages])
         _launch(dev, "focr_beam_reorder", parents.data_ptr(), table.data_ptr(), kv_lens.data_ptr(), spare.data_ptr(),
-                table_out.data_ptr(), spare_out.data_ptr(), ptrs, len(pages), groups, beams, heads, dim, page, table.shape[1],
-                num_pages, _DTYPES[pages[0].dtype])
+                table_out.data_ptr(), spare_out.data_ptr(), ptrs, len(pages), groups, beams, heads, dim, page, tshape[1],
+                num_pages, _DTYPES[dt])
     return table_out, spare_out
 
 
@@ -238,8 +252,8 @@ class PagedCache:
 
     def __init__(self, seqs, max_len, heads, dim, layers=1, page=16, dtype=torch.float32, device="cuda"):
         _need(seqs > 0 and max_len > 0 and heads > 0 and layers > 0, "seqs, max_len, heads and layers must be positive")
-        _need(8 <= page <= 1024 and page & (page - 1) == 0, "page must be a power of two from 8 to 1024, got %d" % page)
-        _need(dim in (64, 128, 256) and dtype in _DTYPES, "head dim must be 64, 128 or 256, the type fp32, bf16 or fp16")
+        _need(page in _PAGES, "page must be a power of two from 8 to 1024, got %d", page)
+        _need(dim in _DIMS and dtype in _DTYPES, "head dim must be 64, 128 or 256, the type fp32, bf16 or fp16")
         per = -(-max_len // page)
         num = seqs * (per + 1)
         _need(num < 2 ** 31, "more pages than int32 numbers")
@@ -252,7 +266,7 @@ class PagedCache:
 
     def advance(self, n):
         """n more tokens for every sequence (their keys and values follow with `append`)"""
-        _need(n >= 0 and self.length + n <= self.max_len, "%d + %d tokens in a cache of %d" % (self.length, n, self.max_len))
+        _need(n >= 0 and self.length + n <= self.max_len, "%d + %d tokens in a cache of %d", self.length, n, self.max_len)
         self.length += n
         self.kv_lens += n
 
