@@ -11,95 +11,326 @@
 // normaliser is not finite, ranks as -inf.  Continuations of different beams may differ by less than fp32 resolves, so the
 // normaliser and the comparison are held in 64 bits; the scores that go out are rounded once.
 // ======================================================================================================================
-__device__ __forceinline__ float bs_load(const void* p, long i, int dtype) {
-  if (dtype == FOCR_DT_F32) return ((const float*)p)[i];
-  if (dtype == FOCR_DT_BF16) return (float)((const __bf16*)p)[i];
-  return (float)((const _Float16*)p)[i];
-}
-struct BsBest {
-  double c;
-  long i;
-};
-__device__ __forceinline__ bool bs_before(double ca, long ia, double cb, long ib) { return ca > cb || (ca == cb && ia < ib); }
+//
+// One pass over the logits: a wave takes a segment of a row, 2048 values at a time in registers, and keeps
+//   * per lane the running maximum and the sum of exp(x - maximum) in 64 bits.  The exponential is 16 full-rate fp64 operations
+//     (a multiple of ln 2 taken off by a rounding addition, Taylor's polynomial of degree 9 on the rest: 7e-12), about what the
+//     loads of 16-bit logits cost in time; a hardware exp2 in fp32 would be off by 1e-7, as far apart as neighbours can be;
+//   * its n best as a list across the lanes (lane i: the i-th best), sorted by one 64-bit key: the value's bits in an order that
+//     compares as integers, then the complement of the index.  Almost no value passes the n-th best; one that does is placed by a
+//     ballot and a shift of one lane.  The first chunk starts from the n-th largest of the lanes' maxima as its threshold.
+// Segments start at fixed indices and lanes take fixed indices of them whatever the row's alignment, so equal rows have
+// equal sums.  A second pass over K x segments lists of n joins them (in the same block where a batch entry is small).
+#define BS_CHUNK 2048
+#define BS_MAX 64                     // beams, and candidates asked for
+#define BS_WAVES 16                   // of the one-launch form
+typedef unsigned long long u64_t;
+typedef __attribute__((ext_vector_type(4))) uint32_t bs_u32x4;
+typedef __attribute__((ext_vector_type(4), aligned(2))) uint32_t bs_u32x4_any;      // 16 bytes at any element's address
 
-__global__ __launch_bounds__(256) void beam_select_kernel(const void* __restrict__ logits, long ldb, long ldk,
-                                                          const float* __restrict__ scores, const uint8_t* __restrict__ fin,
-                                                          float* __restrict__ out_scores, int* __restrict__ out_parents,
-                                                          long long* __restrict__ out_tokens, uint8_t* __restrict__ out_fin,
-                                                          int beams, int vocab, int n, int eos, int dtype) {
-  __shared__ double add[64];          // s_k - normaliser; NaN: the beam is dead
-  __shared__ BsBest best[4];
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  for (int k = wave; k < beams; k += 4) {
-    const long row = b * ldb + k * ldk;
+struct BsStat {                       // of a segment
+  double sum;                         // of exp(x - max)
+  float max;                          // NaN: the segment holds one
+};
+
+__device__ __forceinline__ uint32_t bs_order(float x) {           // -inf < .. < +inf as integers; both zeros alike, NaN as -inf
+  const uint32_t b = __float_as_uint(x != x ? -INFINITY : x + 0.f);
+  return b >> 31 ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float bs_value(u64_t key) {
+  const uint32_t o = (uint32_t)(key >> 32);
+  return __uint_as_float(o >> 31 ? o & 0x7fffffffu : ~o);
+}
+__device__ __forceinline__ int bs_index(u64_t key) { return (int)~(uint32_t)key; }
+__device__ __forceinline__ u64_t bs_key(float x, int v) { return (u64_t)bs_order(x) << 32 | (uint32_t)~v; }
+
+__device__ __forceinline__ double bs_exp(double t) {              // t <= 0; exp(-700) stands for everything below
+  t = fmax(t, -700.0);
+  const double u = fma(t, 1.4426950408889634, 6755399441055744.0);           // 1.5 * 2^52: rounds to an integer, kept in the low word
+  const double r = fma(u - 6755399441055744.0, -0.6931471805599453, t);
+  double p = 1.0 / 362880;
+  p = fma(p, r, 1.0 / 40320);
+  p = fma(p, r, 1.0 / 5040);
+  p = fma(p, r, 1.0 / 720);
+  p = fma(p, r, 1.0 / 120);
+  p = fma(p, r, 1.0 / 24);
+  p = fma(p, r, 1.0 / 6);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  return __hiloint2double(__double2hiint(p) + (__double2loint(u) << 20), __double2loint(p));
+}
+
+__device__ __forceinline__ u64_t bs_lane(u64_t x, int l) {
+  return (u64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), l) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)x, l);
+}
+// key (the same in all lanes) into the sorted list across the lanes; what falls off its end is lost
+__device__ __forceinline__ void bs_insert(u64_t& list, u64_t key, int lane) {
+  const int at = __popcll(__ballot(list > key));
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(list >> 32), 0x138, 0xf, 0xf, false);      // from the lane below
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)list, 0x138, 0xf, 0xf, false);
+  list = lane < at ? list : lane == at ? key : (u64_t)hi << 32 | lo;
+}
+
+template <typename T>
+__device__ __forceinline__ void bs_scan(const T* row, int v0, int v1, int n, int lane, u64_t& list, BsStat& stat) {
+  constexpr int E = 16 / sizeof(T), L = BS_CHUNK / (64 * E);      // values of a load, loads of a chunk
+  list = 0;                                                       // below every value's key
+  float m = -INFINITY;
+  double sum = 0.0;
+  bool nan = false;
+  float thr = -INFINITY;
+  bool first = true;
+  for (int base = v0; base < v1; base += BS_CHUNK) {
+    float x[L * E];
+#pragma unroll
+    for (int j = 0; j < L; ++j) {
+      const int v = base + (j * 64 + lane) * E;
+      if (v + E <= v1) {
+        const bs_u32x4 w = *(const bs_u32x4_any*)(row + v);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          if constexpr (sizeof(T) == 4) x[j * E + e] = __uint_as_float(w[e]);
+          else x[j * E + e] = (float)__builtin_bit_cast(T, (uint16_t)(w[e / 2] >> (16 * (e & 1))));
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[j * E + e] = v + e < v1 ? (float)row[v + e] : -INFINITY;
+      }
+    }
+    float cm = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < L * E; ++i) {
+      nan |= x[i] != x[i];
+      cm = fmaxf(cm, x[i]);
+    }
+    if (cm > m) {
+      sum *= bs_exp((double)m - (double)cm);                      // (-inf before the first values: the sum is 0)
+      m = cm;
+    }
+    const double ref = m == -INFINITY ? 0.0 : (double)m;
+#pragma unroll
+    for (int i = 0; i < L * E; ++i) sum += bs_exp((double)x[i] - ref);      // (-inf: 1e-304, nothing beside the maximum's 1)
+
+    if (first && v1 - v0 > 256) {                                 // the n-th largest of 64 values that are there: a bound
+      int rank = 0;
+#pragma unroll
+      for (int j = 0; j < 64; ++j) {
+        const float y = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(cm), j));
+        rank += y > cm || (y == cm && j < lane);
+      }
+      thr = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(cm), __builtin_ctzll(__ballot(rank == n - 1))));
+    }
+    // against the list's own n-th best an equal value that comes later is no better; in the first chunk it may be
+#pragma unroll
+    for (int i = 0; i < L * E; ++i) {
+      const int v = base + ((i / E) * 64 + lane) * E + i % E;
+      u64_t pass = __ballot((first ? x[i] >= thr : x[i] > thr) && v < v1);
+      while (pass) {
+        const int l = __builtin_ctzll(pass);
+        pass &= pass - 1;
+        const float y = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x[i]), l));
+        bs_insert(list, bs_key(y, v - lane * E + l * E), lane);
+        const u64_t last = bs_lane(list, n - 1);
+        if (last) thr = fmaxf(thr, bs_value(last));
+      }
+    }
+    first = first && bs_lane(list, n - 1) == 0;                   // a short first chunk: the list is not full yet
+  }
+  const float mx = wave_max(m);
+  sum = m == -INFINITY ? 0.0 : sum * bs_exp((double)m - (double)mx);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  stat.max = __ballot(nan) ? NAN : mx;
+  stat.sum = sum;
+}
+
+struct BsArgs {
+  const void* logits;
+  long ldb, ldk;
+  const float* scores;
+  const uint8_t* fin;
+  float* out_scores;
+  int* out_parents;
+  long long* out_tokens;
+  uint8_t* out_fin;
+  u64_t* lists;                       // [batch][beams][parts][n]
+  BsStat* stats;                      // [batch][beams][parts]
+  int beams, vocab, n, eos, parts, seg;
+};
+
+__device__ __forceinline__ bool bs_before(double ca, int ia, double cb, int ib) { return ca > cb || (ca == cb && ia < ib); }
+
+// Joins the lists of a batch entry (waves: of the block; lists / stats of this entry).  rc / rv [beams][n]: the rows' candidates
+__device__ __forceinline__ void bs_join(const BsArgs& a, int b, const u64_t* lists, const BsStat* stats, double* rc, int* rv,
+                                        int waves) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = a.n;
+  const int have = n < a.vocab ? n : a.vocab;                     // candidates of a row
+  for (int k = wave; k < a.beams; k += waves) {
+    u64_t list = lane < n ? lists[(long)k * a.parts * n + lane] : 0;
+    for (int p = 1; p < a.parts; ++p) {
+      const u64_t other = lane < n ? lists[((long)k * a.parts + p) * n + lane] : 0;
+      for (int i = 0; i < n; ++i) {
+        const u64_t key = bs_lane(other, i);
+        if (key <= bs_lane(list, n - 1)) break;
+        bs_insert(list, key, lane);
+      }
+    }
     float m = -INFINITY;
+    double sum = 0.0;
     bool nan = false;
-    for (int v = lane; v < vocab; v += 64) {
-      const float x = bs_load(logits, row + v, dtype);
+    for (int p = lane; p < a.parts; p += 64) {
+      const float x = stats[k * a.parts + p].max;
       nan |= x != x;
       m = fmaxf(m, x);
     }
     m = wave_max(m);
-    nan = __ballot(nan) != 0;
-    double sum = 0.0;
-    for (int v = lane; v < vocab; v += 64) sum += exp((double)bs_load(logits, row + v, dtype) - (double)m);
+    for (int p = lane; p < a.parts; p += 64) {
+      const BsStat st = stats[k * a.parts + p];
+      if (st.max > -INFINITY) sum += st.sum * bs_exp((double)st.max - (double)m);
+    }
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    const float s = scores[b * beams + k];
-    double a = (double)s - ((double)m + log(sum));
-    if (fin && fin[b * beams + k]) a = (double)s;
-    else if (nan || !isfinite(m)) a = NAN;
-    if (!isfinite(s)) a = NAN;
-    if (lane == 0) add[k] = a;
+    const float s = a.scores[b * a.beams + k];
+    const bool done = a.fin && a.fin[b * a.beams + k];
+    const bool live = isfinite(s) && (done || (!__ballot(nan) && isfinite(m)));
+    double c = -INFINITY;
+    int v = lane;
+    if (live && done) {                                           // (eos, s), then the others as they come
+      v = lane == 0 ? a.eos : lane <= a.eos ? lane - 1 : lane;
+      if (lane == 0) c = (double)s;
+    } else if (live) {
+      v = bs_index(list);
+      c = (double)s - ((double)m + log(sum)) + (double)bs_value(list);
+    }
+    // in order of (candidate, index): 64 bits may round different logits to one candidate
+    int at = 0;
+    for (int j = 0; j < have; ++j) {
+      const double cj = __shfl(c, j, 64);
+      const int vj = __shfl(v, j, 64);
+      at += j != lane && bs_before(cj, vj, c, v);
+    }
+    if (lane < have) {
+      rc[k * n + at] = c;
+      rv[k * n + at] = v;
+    }
   }
   __syncthreads();
-  double pc = INFINITY;
-  long pi = -1;
-  const long total = (long)beams * vocab;
-  for (int r = 0; r < n; ++r) {
-    double bc = -INFINITY;
-    long bi = INT64_MAX;
-    for (long i = tid; i < total; i += 256) {
-      const int k = (int)(i / vocab), v = (int)(i - (long)k * vocab);
-      double c;
-      if (fin && fin[b * beams + k]) c = v == eos ? add[k] : (double)-INFINITY;
-      else c = add[k] + (double)bs_load(logits, b * ldb + k * ldk + v, dtype);
-      if (!(c == c)) c = -INFINITY;
-      if (bs_before(pc, pi, c, i) && bs_before(c, i, bc, bi)) bc = c, bi = i;
+  // a candidate's place: its place in its own row plus, by bisection, how many of every other row come before it
+  for (int x = tid; x < a.beams * have; x += waves * 64) {
+    const int k = x / have, i = x - k * have;
+    const double c = rc[k * n + i];
+    const int v = rv[k * n + i];
+    int at = i;
+    for (int r = 0; r < a.beams && at < n; ++r) {
+      if (r == k) continue;
+      int lo = 0, hi = have;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        const double cm = rc[r * n + mid];
+        if (cm > c || (cm == c && r < k)) lo = mid + 1;
+        else hi = mid;
+      }
+      at += lo;
     }
-    for (int o = 32; o > 0; o >>= 1) {
-      const double c = __shfl_xor(bc, o, 64);
-      const long i = __shfl_xor(bi, o, 64);
-      if (bs_before(c, i, bc, bi)) bc = c, bi = i;
-    }
-    if (lane == 0) best[wave] = {bc, bi};
-    __syncthreads();
-    pc = best[0].c, pi = best[0].i;
-    for (int w = 1; w < 4; ++w)
-      if (bs_before(best[w].c, best[w].i, pc, pi)) pc = best[w].c, pi = best[w].i;
-    __syncthreads();
-    if (tid == 0) {
-      const int k = (int)(pi / vocab), v = (int)(pi - (long)k * vocab);
-      out_scores[b * n + r] = (float)pc;
-      out_parents[b * n + r] = k;
-      out_tokens[b * n + r] = v;
-      out_fin[b * n + r] = (fin && fin[b * beams + k]) || v == eos;
+    if (at < n) {
+      a.out_scores[b * n + at] = (float)c;
+      a.out_parents[b * n + at] = k;
+      a.out_tokens[b * n + at] = v;
+      a.out_fin[b * n + at] = (a.fin && a.fin[b * a.beams + k]) || v == a.eos;
     }
   }
 }
 
-extern "C" long focr_beam_select_ws_bytes(int batch, int beams, int vocab, int n, int dtype) { return 0; }
+// a whole batch entry in a block: wave (beam, segment)
+template <typename T>
+__global__ __launch_bounds__(64 * BS_WAVES) void beam_select_kernel(BsArgs a) {
+  __shared__ u64_t lists[BS_WAVES * BS_MAX];
+  __shared__ BsStat stats[BS_WAVES];
+  __shared__ double rc[BS_WAVES * BS_MAX];
+  __shared__ int rv[BS_WAVES * BS_MAX];
+  const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, k = wave / a.parts, p = wave - k * a.parts;
+  u64_t list;
+  BsStat st;
+  const int v0 = p * a.seg, v1 = v0 + a.seg < a.vocab ? v0 + a.seg : a.vocab;
+  bs_scan((const T*)a.logits + b * a.ldb + k * a.ldk, v0, v1, a.n, lane, list, st);
+  if (lane < a.n) lists[wave * a.n + lane] = list;
+  if (lane == 0) stats[wave] = st;
+  __syncthreads();
+  bs_join(a, b, lists, stats, rc, rv, a.beams * a.parts);
+}
+
+// the two-launch form
+template <typename T>
+__global__ __launch_bounds__(256) void beam_scan_kernel(BsArgs a, int waves) {
+  const int lane = threadIdx.x & 63, w = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (w >= waves) return;
+  const int p = w % a.parts, row = w / a.parts, b = row / a.beams, k = row - b * a.beams;
+  u64_t list;
+  BsStat st;
+  const int v0 = p * a.seg, v1 = v0 + a.seg < a.vocab ? v0 + a.seg : a.vocab;
+  bs_scan((const T*)a.logits + b * a.ldb + k * a.ldk, v0, v1, a.n, lane, list, st);
+  if (lane < a.n) a.lists[(long)w * a.n + lane] = list;
+  if (lane == 0) a.stats[w] = st;
+}
+__global__ __launch_bounds__(256) void beam_join_kernel(BsArgs a) {
+  extern __shared__ double bs_rc[];                               // [beams][n], then the indices
+  const long rows = (long)blockIdx.x * a.beams * a.parts;
+  bs_join(a, blockIdx.x, a.lists + rows * a.n, a.stats + rows, bs_rc, (int*)(bs_rc + a.beams * a.n), 4);
+}
+
+// One launch with a block per batch entry while an entry has at most 64 K logits (5 x 6625 fp32, 64 entries: see below), else the
+// rows are cut into segments of whole chunks, about 4096 waves in all, and joined by a second launch.
+struct BsPlan {
+  bool one;
+  int parts, seg;
+};
+#ifndef BS_ONE
+#define BS_ONE 65536
+#endif
+static BsPlan bs_plan(int batch, int beams, int vocab) {
+  const int chunks = (vocab + BS_CHUNK - 1) / BS_CHUNK;
+  BsPlan p;
+  p.one = beams <= BS_WAVES && (long)beams * vocab <= BS_ONE;
+  const long want = p.one ? BS_WAVES / beams : 4096 / ((long)batch * beams);
+  const int per = want < 1 ? chunks : (int)((chunks + want - 1) / want);
+  p.seg = per * BS_CHUNK;
+  p.parts = (chunks + per - 1) / per;
+  return p;
+}
+
+extern "C" long focr_beam_select_ws_bytes(int batch, int beams, int vocab, int n, int dtype) {
+  if (batch <= 0 || beams <= 0 || vocab <= 0 || n <= 0) return 0;
+  const BsPlan p = bs_plan(batch, beams, vocab);
+  return p.one ? 0 : (long)batch * beams * p.parts * (n * (long)sizeof(u64_t) + (long)sizeof(BsStat));
+}
 
 extern "C" int focr_beam_select(const void* logits, long ldb, long ldk, const float* scores, const uint8_t* finished,
                                 float* out_scores, int* out_parents, long long* out_tokens, uint8_t* out_finished, void* ws,
                                 long ws_bytes, int batch, int beams, int vocab, int n, int eos, int dtype, void* stream) {
   FOCR_CHECK_ARG(dtype == FOCR_DT_F32 || dtype == FOCR_DT_BF16 || dtype == FOCR_DT_F16, "dtype must be fp32, bf16 or fp16");
-  FOCR_CHECK_ARG(batch >= 0 && beams > 0 && beams <= 64 && vocab > 0, "beams must be 1 to 64, vocab positive");
-  FOCR_CHECK_ARG(n > 0 && n <= 64 && n <= (long)beams * vocab, "n must be 1 to 64 and at most beams * vocab");
+  FOCR_CHECK_ARG(batch >= 0 && beams > 0 && beams <= BS_MAX && vocab > 0 && vocab < INT32_MAX - 2 * BS_CHUNK,
+                 "beams must be 1 to 64, vocab positive");
+  FOCR_CHECK_ARG(n > 0 && n <= BS_MAX && n <= (long)beams * vocab, "n must be 1 to 64 and at most beams * vocab");
   FOCR_CHECK_ARG(!finished || (eos >= 0 && eos < vocab), "finished beams need an eos inside the vocabulary");
   if (batch == 0) return FOCR_OK;
   FOCR_CHECK_ARG(logits && scores && out_scores && out_parents && out_tokens && out_finished, "null pointer");
-  hipLaunchKernelGGL(beam_select_kernel, dim3(batch), dim3(256), 0, (hipStream_t)stream, logits, ldb, ldk, scores, finished,
-                     out_scores, out_parents, out_tokens, out_finished, beams, vocab, n, eos, dtype);
+  const BsPlan p = bs_plan(batch, beams, vocab);
+  const long rows = (long)batch * beams * p.parts;
+  FOCR_CHECK_ARG(rows <= INT32_MAX - 4, "too many rows for one launch");
+  FOCR_CHECK_ARG(p.one || (ws && ((uintptr_t)ws & 7) == 0 && ws_bytes >= focr_beam_select_ws_bytes(batch, beams, vocab, n, dtype)),
+                 "workspace missing or too small (focr_beam_select_ws_bytes)");
+  BsArgs a = {logits, ldb, ldk, scores, finished, out_scores, out_parents, out_tokens, out_finished, (u64_t*)ws,
+              p.one ? nullptr : (BsStat*)((u64_t*)ws + rows * n), beams, vocab, n, eos, p.parts, p.seg};
+  const hipStream_t st = (hipStream_t)stream;
+  if (p.one) {
+    auto kern = dtype == FOCR_DT_F32 ? beam_select_kernel<float> : dtype == FOCR_DT_BF16 ? beam_select_kernel<__bf16> : beam_select_kernel<_Float16>;
+    hipLaunchKernelGGL(kern, dim3(batch), dim3(64 * beams * p.parts), 0, st, a);
+  } else {
+    auto kern = dtype == FOCR_DT_F32 ? beam_scan_kernel<float> : dtype == FOCR_DT_BF16 ? beam_scan_kernel<__bf16> : beam_scan_kernel<_Float16>;
+    hipLaunchKernelGGL(kern, dim3(cdiv(rows, 4)), dim3(256), 0, st, a, (int)rows);
+    FOCR_LAUNCH_CHECK();
+    hipLaunchKernelGGL(beam_join_kernel, dim3(batch), dim3(256), beams * n * 12, st, a);
+  }
   FOCR_LAUNCH_CHECK();
   return FOCR_OK;
 }
