@@ -13,17 +13,19 @@
 // ======================================================================================================================
 //
 // One pass over the logits: a wave takes a segment of a row, 2048 values at a time in registers, and keeps
-//   * per lane the running maximum and the sum of exp(x - maximum) in 64 bits.  The exponential is 16 full-rate fp64 operations
-//     (a multiple of ln 2 taken off by a rounding addition, Taylor's polynomial of degree 9 on the rest: 7e-12), about what the
+//   * per lane the running maximum and the sum of exp(x - maximum) in 64 bits.  The exponential is 13 full-rate fp64 operations
+//     (a multiple of ln 2 taken off by a rounding addition, a polynomial of degree 7 on the rest: 6e-11), about what the
 //     loads of 16-bit logits cost in time; a hardware exp2 in fp32 would be off by 1e-7, as far apart as neighbours can be;
-//   * its n best as a list across the lanes (lane i: the i-th best), sorted by one 64-bit key: the value's bits in an order that
-//     compares as integers, then the complement of the index.  Almost no value passes the n-th best; one that does is placed by a
-//     ballot and a shift of one lane.  The first chunk starts from the n-th largest of the lanes' maxima as its threshold.
+//   * a buffer of the values that may be among its n best, as 64-bit keys: the value's bits in an order that compares as integers,
+//     then the complement of the index.  The n-th largest of the lanes' running maxima is a lower bound of the n-th best, so
+//     little more than n values pass; they are appended by ballot, all lanes at once, and put in order at the end (placing each
+//     in a sorted list as it came took 14 us of the scan's 41 at 64 x 8 x 50001).
 // Segments start at fixed indices and lanes take fixed indices of them whatever the row's alignment, so equal rows have
 // equal sums.  A second pass over K x segments lists of n joins them (in the same block where a batch entry is small).
 #define BS_CHUNK 2048
 #define BS_MAX 64                     // beams, and candidates asked for
 #define BS_WAVES 16                   // of the one-launch form
+#define BS_BUF 256                    // keys a wave gathers: more than twice BS_MAX
 typedef unsigned long long u64_t;
 typedef __attribute__((ext_vector_type(4))) uint32_t bs_u32x4;
 typedef __attribute__((ext_vector_type(4), aligned(2))) uint32_t bs_u32x4_any;      // 16 bytes at any element's address
@@ -48,17 +50,27 @@ __device__ __forceinline__ double bs_exp(double t) {              // t <= 0; exp
   t = fmax(t, -700.0);
   const double u = fma(t, 1.4426950408889634, 6755399441055744.0);           // 1.5 * 2^52: rounds to an integer, kept in the low word
   const double r = fma(u - 6755399441055744.0, -0.6931471805599453, t);
-  double p = 1.0 / 362880;
-  p = fma(p, r, 1.0 / 40320);
-  p = fma(p, r, 1.0 / 5040);
-  p = fma(p, r, 1.0 / 720);
-  p = fma(p, r, 1.0 / 120);
-  p = fma(p, r, 1.0 / 24);
-  p = fma(p, r, 1.0 / 6);
-  p = fma(p, r, 0.5);
-  p = fma(p, r, 1.0);
-  p = fma(p, r, 1.0);
+  double p = 0.00019907582591804609;                              // interpolates exp at the Chebyshev nodes of |r| <= ln 2 / 2
+  p = fma(p, r, 0.0013948590286876341);
+  p = fma(p, r, 0.008333283518767049);
+  p = fma(p, r, 0.04166621813971032);
+  p = fma(p, r, 0.16666666786380446);
+  p = fma(p, r, 0.5000000107793876);
+  p = fma(p, r, 0.9999999999955055);
+  p = fma(p, r, 0.9999999999595294);
   return __hiloint2double(__double2hiint(p) + (__double2loint(u) << 20), __double2loint(p));
+}
+// the largest value of the wave, in every lane: lane crossings inside the vector unit
+__device__ __forceinline__ float bs_wave_max(float x) {
+#define BS_STEP(ctrl) x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp((int)0xff800000, __float_as_int(x), ctrl, 0xf, 0xf, false)))
+  BS_STEP(0x111);
+  BS_STEP(0x112);
+  BS_STEP(0x114);
+  BS_STEP(0x118);
+  BS_STEP(0x142);
+  BS_STEP(0x143);
+#undef BS_STEP
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
 }
 
 __device__ __forceinline__ u64_t bs_lane(u64_t x, int l) {
@@ -72,72 +84,137 @@ __device__ __forceinline__ void bs_insert(u64_t& list, u64_t key, int lane) {
   list = lane < at ? list : lane == at ? key : (u64_t)hi << 32 | lo;
 }
 
-template <typename T>
-__device__ __forceinline__ void bs_scan(const T* row, int v0, int v1, int n, int lane, u64_t& list, BsStat& stat) {
-  constexpr int E = 16 / sizeof(T), L = BS_CHUNK / (64 * E);      // values of a load, loads of a chunk
-  list = 0;                                                       // below every value's key
-  float m = -INFINITY;
+// The n best of the buffer's cnt keys to out[0 .. n) in order (0 where there are fewer): every key finds its place by counting
+// the ones above it
+__device__ __forceinline__ void bs_trim(const u64_t* buf, int cnt, int n, int lane, u64_t* out) {
+  if (lane >= cnt && lane < n) out[lane] = 0;
+  for (int i = 0; i < cnt; i += 64) {
+    const u64_t mine = i + lane < cnt ? buf[i + lane] : 0;
+    int at = 0;
+    for (int j = 0; j < cnt; j += 64) {
+      const u64_t other = j + lane < cnt ? buf[j + lane] : 0;
+      const int m = cnt - j < 64 ? cnt - j : 64;
+      for (int e = 0; e < m; ++e) at += bs_lane(other, e) > mine;
+    }
+    if (i + lane < cnt && at < n) out[at] = mine;
+  }
+  __builtin_amdgcn_wave_barrier();
+}
+
+template <typename T, int L>          // L loads of 16 bytes a lane make a chunk
+__device__ __forceinline__ void bs_scan(const T* row, int v0, int v1, int n, int lane, u64_t* buf, u64_t* best, BsStat& stat) {
+  constexpr int E = 16 / sizeof(T), CHUNK = L * 64 * E, G = L * E < 8 ? L * E : 8;      // G: values compared together
+  float m = -INFINITY, thr = -INFINITY;
   double sum = 0.0;
-  bool nan = false;
-  float thr = -INFINITY;
-  bool first = true;
-  for (int base = v0; base < v1; base += BS_CHUNK) {
+  bool nan = false, ahead = false;
+  int cnt = 0;
+  bs_u32x4 w[L];
+  auto load = [&](int base) {
+#pragma unroll
+    for (int j = 0; j < L; ++j) w[j] = *(const bs_u32x4_any*)(row + base + (j * 64 + lane) * E);
+  };
+  for (int base = v0; base < v1; base += CHUNK) {
     float x[L * E];
+    if (base + CHUNK <= v1) {
+      if (!ahead) load(base);
 #pragma unroll
-    for (int j = 0; j < L; ++j) {
-      const int v = base + (j * 64 + lane) * E;
-      if (v + E <= v1) {
-        const bs_u32x4 w = *(const bs_u32x4_any*)(row + v);
+      for (int i = 0; i < L * E; ++i) {
+        if constexpr (sizeof(T) == 4) x[i] = __uint_as_float(w[i / E][i % E]);
+        else x[i] = (float)__builtin_bit_cast(T, (uint16_t)(w[i / E][i % E / 2] >> (16 * (i & 1))));
+        nan |= x[i] != x[i];
+      }
+    } else {
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          if constexpr (sizeof(T) == 4) x[j * E + e] = __uint_as_float(w[e]);
-          else x[j * E + e] = (float)__builtin_bit_cast(T, (uint16_t)(w[e / 2] >> (16 * (e & 1))));
+      for (int i = 0; i < L * E; ++i) {
+        const int v = base + ((i / E) * 64 + lane) * E + i % E;
+        x[i] = NAN;                                               // none: passes no comparison, adds nothing
+        if (v < v1) {
+          x[i] = (float)row[v];
+          nan |= x[i] != x[i];
         }
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) x[j * E + e] = v + e < v1 ? (float)row[v + e] : -INFINITY;
       }
     }
-    float cm = -INFINITY;
+    ahead = base + 2 * CHUNK <= v1;
+    if (ahead) load(base + CHUNK);                                // under this chunk's arithmetic
+    float gm[L * E / G], cm = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < L * E; ++i) {
-      nan |= x[i] != x[i];
-      cm = fmaxf(cm, x[i]);
+    for (int g = 0; g < L * E / G; ++g) {
+      gm[g] = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < G; ++i) gm[g] = fmaxf(gm[g], x[g * G + i]);
+      cm = fmaxf(cm, gm[g]);
     }
+    const bool better = __ballot(cm >= thr) != 0;
     if (cm > m) {
       sum *= bs_exp((double)m - (double)cm);                      // (-inf before the first values: the sum is 0)
       m = cm;
     }
     const double ref = m == -INFINITY ? 0.0 : (double)m;
 #pragma unroll
-    for (int i = 0; i < L * E; ++i) sum += bs_exp((double)x[i] - ref);      // (-inf: 1e-304, nothing beside the maximum's 1)
-
-    if (first && v1 - v0 > 256) {                                 // the n-th largest of 64 values that are there: a bound
-      int rank = 0;
-#pragma unroll
-      for (int j = 0; j < 64; ++j) {
-        const float y = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(cm), j));
-        rank += y > cm || (y == cm && j < lane);
-      }
-      thr = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(cm), __builtin_ctzll(__ballot(rank == n - 1))));
-    }
-    // against the list's own n-th best an equal value that comes later is no better; in the first chunk it may be
-#pragma unroll
     for (int i = 0; i < L * E; ++i) {
-      const int v = base + ((i / E) * 64 + lane) * E + i % E;
-      u64_t pass = __ballot((first ? x[i] >= thr : x[i] > thr) && v < v1);
-      while (pass) {
-        const int l = __builtin_ctzll(pass);
-        pass &= pass - 1;
-        const float y = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x[i]), l));
-        bs_insert(list, bs_key(y, v - lane * E + l * E), lane);
-        const u64_t last = bs_lane(list, n - 1);
-        if (last) thr = fmaxf(thr, bs_value(last));
+      sum += bs_exp((double)x[i] - ref);                          // (-inf: 1e-304, nothing beside the maximum's 1)
+      if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);          // four chains at a time fill the pipe; more only take registers
+    }
+    if (!better) continue;
+
+    if (v1 - v0 > 256) {                                          // the n-th largest of the lanes' maxima: values that are there
+      float t = -INFINITY;
+      if (n <= 16) {
+        float y = m;
+        for (int r = 0; r < n; ++r) {
+          t = bs_wave_max(y);
+          if (lane == __builtin_ctzll(__ballot(y == t) | 1ull << 63)) y = -INFINITY;
+        }
+      } else {
+        int rank = 0;
+#pragma unroll 8
+        for (int j = 0; j < 64; ++j) {
+          const float y = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m), j));
+          rank += y > m || (y == m && j < lane);
+        }
+        t = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m), __builtin_ctzll(__ballot(rank == n - 1) | 1ull << 63)));
+      }
+      thr = fmaxf(thr, t);
+    }
+    const int before = cnt;
+#pragma unroll
+    for (int g = 0; g < L * E / G; ++g) {
+      if (!__ballot(gm[g] >= thr)) continue;
+#pragma unroll
+      for (int i = g * G; i < g * G + G; ++i) {
+        const bool take = x[i] >= thr;
+        const u64_t pass = __ballot(take);
+        if (!pass) continue;
+        if (take && cnt + __popcll(pass) <= BS_BUF)
+          buf[cnt + __builtin_amdgcn_mbcnt_hi((uint32_t)(pass >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)pass, 0))] =
+              bs_key(x[i], base + ((i / E) * 64 + lane) * E + i % E);
+        cnt += __popcll(pass);
       }
     }
-    first = first && bs_lane(list, n - 1) == 0;                   // a short first chunk: the list is not full yet
+    __builtin_amdgcn_wave_barrier();
+    if (cnt > BS_BUF / 2) {
+      // Rarely (many equal values, or ever better ones): the buffer goes back to its n best; if it ran over, this chunk's values
+      // are gone through again, 64 at a time, and placed one by one in the sorted list
+      const bool over = cnt > BS_BUF;
+      bs_trim(buf, over ? before : cnt, n, lane, best);
+      u64_t list = lane < n ? best[lane] : 0;
+      for (int v = base + lane; over && v - lane < v1 && v - lane < base + CHUNK; v += 64) {
+        const u64_t key = v < v1 ? bs_key((float)row[v], v) : 0;
+        u64_t pass = __ballot(key > bs_lane(list, n - 1));
+        while (pass) {
+          const int l = __builtin_ctzll(pass);
+          pass &= pass - 1;
+          bs_insert(list, bs_lane(key, l), lane);
+        }
+      }
+      if (lane < n) buf[lane] = list;
+      cnt = __popcll(__ballot(lane < n && list != 0));
+      if (cnt == n) thr = fmaxf(thr, bs_value(bs_lane(list, n - 1)));
+      __builtin_amdgcn_wave_barrier();
+    }
   }
-  const float mx = wave_max(m);
+  bs_trim(buf, cnt, n, lane, best);
+  const float mx = bs_wave_max(m);
   sum = m == -INFINITY ? 0.0 : sum * bs_exp((double)m - (double)mx);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
@@ -168,13 +245,18 @@ __device__ __forceinline__ void bs_join(const BsArgs& a, int b, const u64_t* lis
   const int have = n < a.vocab ? n : a.vocab;                     // candidates of a row
   for (int k = wave; k < a.beams; k += waves) {
     u64_t list = lane < n ? lists[(long)k * a.parts * n + lane] : 0;
-    for (int p = 1; p < a.parts; ++p) {
-      const u64_t other = lane < n ? lists[((long)k * a.parts + p) * n + lane] : 0;
-      for (int i = 0; i < n; ++i) {
-        const u64_t key = bs_lane(other, i);
-        if (key <= bs_lane(list, n - 1)) break;
-        bs_insert(list, key, lane);
-      }
+    for (int p0 = 1; p0 < a.parts; p0 += 8) {                     // eight loads at a time, then their turn
+      u64_t other[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        other[j] = lane < n && p0 + j < a.parts ? lists[((long)k * a.parts + p0 + j) * n + lane] : 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        for (int i = 0; i < n; ++i) {
+          const u64_t key = bs_lane(other[j], i);
+          if (key <= bs_lane(list, n - 1)) break;
+          bs_insert(list, key, lane);
+        }
     }
     float m = -INFINITY;
     double sum = 0.0;
@@ -242,18 +324,16 @@ __device__ __forceinline__ void bs_join(const BsArgs& a, int b, const u64_t* lis
 }
 
 // a whole batch entry in a block: wave (beam, segment)
-template <typename T>
+template <typename T, int L>
 __global__ __launch_bounds__(64 * BS_WAVES) void beam_select_kernel(BsArgs a) {
-  __shared__ u64_t lists[BS_WAVES * BS_MAX];
+  __shared__ u64_t buf[BS_WAVES * BS_BUF], lists[BS_WAVES * BS_MAX];
   __shared__ BsStat stats[BS_WAVES];
   __shared__ double rc[BS_WAVES * BS_MAX];
   __shared__ int rv[BS_WAVES * BS_MAX];
   const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, k = wave / a.parts, p = wave - k * a.parts;
-  u64_t list;
   BsStat st;
   const int v0 = p * a.seg, v1 = v0 + a.seg < a.vocab ? v0 + a.seg : a.vocab;
-  bs_scan((const T*)a.logits + b * a.ldb + k * a.ldk, v0, v1, a.n, lane, list, st);
-  if (lane < a.n) lists[wave * a.n + lane] = list;
+  bs_scan<T, L>((const T*)a.logits + b * a.ldb + k * a.ldk, v0, v1, a.n, lane, buf + wave * BS_BUF, lists + wave * a.n, st);
   if (lane == 0) stats[wave] = st;
   __syncthreads();
   bs_join(a, b, lists, stats, rc, rv, a.beams * a.parts);
@@ -261,36 +341,35 @@ __global__ __launch_bounds__(64 * BS_WAVES) void beam_select_kernel(BsArgs a) {
 
 // the two-launch form
 template <typename T>
-__global__ __launch_bounds__(256) void beam_scan_kernel(BsArgs a, int waves) {
-  const int lane = threadIdx.x & 63, w = blockIdx.x * 4 + (threadIdx.x >> 6);
+__global__ __launch_bounds__(256, 4) void beam_scan_kernel(BsArgs a, int waves) {
+  __shared__ u64_t buf[4 * BS_BUF], best[4 * BS_MAX];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = blockIdx.x * 4 + wave;
   if (w >= waves) return;
   const int p = w % a.parts, row = w / a.parts, b = row / a.beams, k = row - b * a.beams;
-  u64_t list;
   BsStat st;
   const int v0 = p * a.seg, v1 = v0 + a.seg < a.vocab ? v0 + a.seg : a.vocab;
-  bs_scan((const T*)a.logits + b * a.ldb + k * a.ldk, v0, v1, a.n, lane, list, st);
-  if (lane < a.n) a.lists[(long)w * a.n + lane] = list;
+  bs_scan<T, BS_CHUNK * sizeof(T) / 1024>((const T*)a.logits + b * a.ldb + k * a.ldk, v0, v1, a.n, lane, buf + wave * BS_BUF,
+                                          best + wave * BS_MAX, st);
+  if (lane < a.n) a.lists[(long)w * a.n + lane] = best[wave * BS_MAX + lane];
   if (lane == 0) a.stats[w] = st;
 }
-__global__ __launch_bounds__(256) void beam_join_kernel(BsArgs a) {
+__global__ __launch_bounds__(64 * BS_WAVES) void beam_join_kernel(BsArgs a, int waves) {
   extern __shared__ double bs_rc[];                               // [beams][n], then the indices
   const long rows = (long)blockIdx.x * a.beams * a.parts;
-  bs_join(a, blockIdx.x, a.lists + rows * a.n, a.stats + rows, bs_rc, (int*)(bs_rc + a.beams * a.n), 4);
+  bs_join(a, blockIdx.x, a.lists + rows * a.n, a.stats + rows, bs_rc, (int*)(bs_rc + a.beams * a.n), waves);
 }
 
-// One launch with a block per batch entry while an entry has at most 64 K logits (5 x 6625 fp32, 64 entries: see below), else the
-// rows are cut into segments of whole chunks, about 4096 waves in all, and joined by a second launch.
+// One launch with a block per batch entry while an entry has at most 16 K logits; else the rows are cut into segments of whole
+// chunks, about 4096 waves in all (64 x 8 x 50001 bf16: 2048 waves 51.6 us, 4096 49.6, 8192 51.2), and joined by a second
+// launch (64 x 5 x 6625 fp32: 18.7 us, in one launch 21.5).
 struct BsPlan {
   bool one;
   int parts, seg;
 };
-#ifndef BS_ONE
-#define BS_ONE 65536
-#endif
 static BsPlan bs_plan(int batch, int beams, int vocab) {
   const int chunks = (vocab + BS_CHUNK - 1) / BS_CHUNK;
   BsPlan p;
-  p.one = beams <= BS_WAVES && (long)beams * vocab <= BS_ONE;
+  p.one = beams <= BS_WAVES && (long)beams * vocab <= 16384;
   const long want = p.one ? BS_WAVES / beams : 4096 / ((long)batch * beams);
   const int per = want < 1 ? chunks : (int)((chunks + want - 1) / want);
   p.seg = per * BS_CHUNK;
@@ -323,13 +402,16 @@ extern "C" int focr_beam_select(const void* logits, long ldb, long ldk, const fl
               p.one ? nullptr : (BsStat*)((u64_t*)ws + rows * n), beams, vocab, n, eos, p.parts, p.seg};
   const hipStream_t st = (hipStream_t)stream;
   if (p.one) {
-    auto kern = dtype == FOCR_DT_F32 ? beam_select_kernel<float> : dtype == FOCR_DT_BF16 ? beam_select_kernel<__bf16> : beam_select_kernel<_Float16>;
+    // a handful of classes: one load a lane, an eighth of the instructions to fetch and run through
+#define BS_KERN(T) (vocab <= 1024 / (int)sizeof(T) ? beam_select_kernel<T, 1> : beam_select_kernel<T, BS_CHUNK * sizeof(T) / 1024>)
+    auto kern = dtype == FOCR_DT_F32 ? BS_KERN(float) : dtype == FOCR_DT_BF16 ? BS_KERN(__bf16) : BS_KERN(_Float16);
     hipLaunchKernelGGL(kern, dim3(batch), dim3(64 * beams * p.parts), 0, st, a);
   } else {
     auto kern = dtype == FOCR_DT_F32 ? beam_scan_kernel<float> : dtype == FOCR_DT_BF16 ? beam_scan_kernel<__bf16> : beam_scan_kernel<_Float16>;
     hipLaunchKernelGGL(kern, dim3(cdiv(rows, 4)), dim3(256), 0, st, a, (int)rows);
     FOCR_LAUNCH_CHECK();
-    hipLaunchKernelGGL(beam_join_kernel, dim3(batch), dim3(256), beams * n * 12, st, a);
+    const int waves = beams < BS_WAVES ? beams : BS_WAVES;
+    hipLaunchKernelGGL(beam_join_kernel, dim3(batch), dim3(64 * waves), beams * n * 12, st, a, waves);
   }
   FOCR_LAUNCH_CHECK();
   return FOCR_OK;
