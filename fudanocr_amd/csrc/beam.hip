@@ -421,9 +421,11 @@ extern "C" int focr_beam_select(const void* logits, long ldb, long ldk, const fl
 // Reordering.  The beams of a group have the same length L; beam j goes on from beam p = parents[j].  Full pages are never
 // written again, so j takes p's table entries for them.  The last, partial page (L % page tokens) will be written by every
 // beam: a j != p gets its own copy, in its spare page, and the page it held before becomes its spare.  So a beam moves at most
-// page - 1 tokens however long the sequence, and no page is allocated or freed.
+// page - 1 tokens however long the sequence, and no page is allocated or freed.  Bound by the bytes moved: 64 x 8 beams, 4 layers of
+// 8 x 128 bf16, pages of 64: 97 us for 205 MB written and as many read, in pieces of 8 KB (a large copy: 4.9 TB/s, this 4.2).
 // ======================================================================================================================
 #define BR_MAX_TENSORS 64
+#define BR_PIECE 1024                 // 16-byte units a block moves (512 .. 2048 and several tensors a block: 97 .. 107 us, see below)
 struct BrPages {
   char* p[BR_MAX_TENSORS];
 };
@@ -433,32 +435,47 @@ __device__ __forceinline__ int br_parent(const int* parents, int slot, int beams
   return p >= 0 && p < beams ? slot / beams * beams + p : slot;          // no such beam: the slot goes on from itself
 }
 
-// grid (16 KB pieces of a page, slot, tensor)
-__global__ __launch_bounds__(256) void beam_copy_pages_kernel(BrPages pages, const int* __restrict__ parents,
+// grid (BR_PIECE units of a page, slot, tensor).  Where the tables that go out are not the ones that come in (table_out), the
+// blocks behind the last tensor write them in the same launch
+__global__ __launch_bounds__(256) void beam_copy_pages_kernel(BrPages pages, int tensors, const int* __restrict__ parents,
                                                               const int* __restrict__ table, const int* __restrict__ lens,
-                                                              const int* __restrict__ spare, int beams, int heads,
-                                                              int row_units, int page_shift, int table_ld, long num_pages) {
+                                                              const int* __restrict__ spare, int* __restrict__ table_out,
+                                                              int* __restrict__ spare_out, int beams, int heads, int row_units,
+                                                              int page_shift, int table_ld, long num_pages) {
   const int slot = blockIdx.y, src_slot = br_parent(parents, slot, beams);
-  if (src_slot == slot) return;
   const int len = lens[slot / beams * beams], full = len >> page_shift, rest = len & ((1 << page_shift) - 1);
-  if (len < 0 || full >= table_ld || rest == 0) return;
+  if ((int)blockIdx.z == tensors) {
+    const bool ok = len >= 0 && (full < table_ld || (full == table_ld && rest == 0)), move = ok && rest && src_slot != slot;
+    const int *own = table + (long)slot * table_ld, *src = table + (long)src_slot * table_ld;
+    for (int col = blockIdx.x * 256 + threadIdx.x; col < table_ld; col += gridDim.x * 256)
+      table_out[(long)slot * table_ld + col] = ok && col < full ? src[col] : move && col == full ? spare[slot] : own[col];
+    if (blockIdx.x == 0 && threadIdx.x == 0) spare_out[slot] = move ? own[full] : spare[slot];
+    return;
+  }
+  if (src_slot == slot || len < 0 || full >= table_ld || rest == 0) return;
   const int from = table[(long)src_slot * table_ld + full], to = spare[slot];
   if (from < 0 || from >= num_pages || to < 0 || to >= num_pages) return;
   const int run = rest * row_units, total = heads * run;                 // 16-byte units
   const long head_units = (long)row_units << page_shift;
-  uint4* base = (uint4*)pages.p[blockIdx.z];
-  const uint4* s = base + (long)from * heads * head_units;
-  uint4* d = base + (long)to * heads * head_units;
-  const int x0 = blockIdx.x * 1024 + threadIdx.x;
+  const long s = (long)from * heads * head_units, d = (long)to * heads * head_units;
+  // head of a unit: x / run by one multiplication where that is exact (m = ceil(2^32 / run): x (m run - 2^32) < x run < 2^32)
+  const uint32_t magic = 0xffffffffu / (uint32_t)run + 1;
+  const bool quick = (uint64_t)total * (uint32_t)run < 1ull << 32 && run > 1;
+  if ((int)blockIdx.x * BR_PIECE >= total) return;
+  const int x0 = blockIdx.x * BR_PIECE + threadIdx.x;
+  long at[BR_PIECE / 256];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int x = x0 + i * 256;
-    if (x < total) {
-      const int h = x / run;
-      const long at = h * head_units + (x - h * run);
-      d[at] = s[at];
-    }
+  for (int i = 0; i < BR_PIECE / 256; ++i) {
+    const int x = x0 + i * 256 < total ? x0 + i * 256 : total - 1, h = quick ? (int)__umulhi((uint32_t)x, magic) : x / run;
+    at[i] = h * head_units + (x - h * run);
   }
+  bs_u32x4* p = (bs_u32x4*)pages.p[blockIdx.z];
+  bs_u32x4 v[BR_PIECE / 256];
+#pragma unroll
+  for (int i = 0; i < BR_PIECE / 256; ++i) v[i] = p[s + at[i]];          // all on their way before the first store
+#pragma unroll
+  for (int i = 0; i < BR_PIECE / 256; ++i)
+    if (x0 + i * 256 < total) p[d + at[i]] = v[i];
 }
 
 // one thread per table column of a group: it reads the column of every beam before it writes one, so the outputs may be the
@@ -497,15 +514,20 @@ extern "C" int focr_beam_reorder(const int* parents, const int* table, const int
   FOCR_CHECK_ARG(parents && table && kv_lens && spare && table_out && spare_out && (pages || !tensors), "null pointer");
   for (int i = 0; i < tensors; ++i) FOCR_CHECK_ARG(pages[i] && ((uintptr_t)pages[i] & 15) == 0, "pages must be 16-byte aligned");
   const int shift = __builtin_ctz(page);
+  const long slots = (long)groups * beams;
+  const bool apart = (table_out + slots * table_ld <= table || table + slots * table_ld <= table_out) &&
+                     (spare_out + slots <= spare || spare + slots <= spare_out);
   for (int i = 0; i < tensors; i += BR_MAX_TENSORS) {
     BrPages b = {};
     const int m = tensors - i < BR_MAX_TENSORS ? tensors - i : BR_MAX_TENSORS;
     for (int j = 0; j < m; ++j) b.p[j] = (char*)pages[i + j];
-    hipLaunchKernelGGL(beam_copy_pages_kernel, dim3(cdiv(page_bytes, 16384), groups * beams, m), dim3(256), 0,
-                       (hipStream_t)stream, b, parents, table, kv_lens, spare, beams, heads, (int)(row_bytes / 16), shift,
-                       table_ld, num_pages);
+    const bool tables = apart && i + m == tensors;
+    hipLaunchKernelGGL(beam_copy_pages_kernel, dim3(cdiv(page_bytes, 16 * BR_PIECE), slots, m + (tables ? 1 : 0)), dim3(256), 0,
+                       (hipStream_t)stream, b, m, parents, table, kv_lens, spare, table_out, spare_out, beams, heads,
+                       (int)(row_bytes / 16), shift, table_ld, num_pages);
     FOCR_LAUNCH_CHECK();
   }
+  if (apart && tensors) return FOCR_OK;
   hipLaunchKernelGGL(beam_tables_kernel, dim3(cdiv(table_ld, 256), groups), dim3(256), beams * 1024, (hipStream_t)stream,
                      parents, table, kv_lens, spare, table_out, spare_out, beams, shift, table_ld);
   FOCR_LAUNCH_CHECK();
