@@ -113,3 +113,12 @@ class Transformer(nn.Module):
         idx = torch.tensor([i * length + j for i, n in enumerate(lens) for j in range(n)], dtype=torch.long)
         probs_res = ops.gather_rows(logits.view(b * length, -1), idx.to(logits.device, non_blocking=True))
         return probs_res, word_attention_map, None
+
+    def beam_search(self, image, beams=4, max_len=26):
+        """the `beams` most likely strings of every image: (tokens int64 [B, beams, max_len], log-probabilities fp32 [B, beams]),
+        best first, closed with '-' (fudanocr_amd/sld/beam.py).  image NCHW [B,1,32,128]; eval mode."""
+        from ..sld import beam
+        with torch.no_grad():
+            feat = self.encoder(image)
+        return beam.search(self, feat, self.embedding_word, self.generator_word, beams, max_len, alphabet.index("-"),
+                           alphabet.index("-"))

@@ -71,3 +71,14 @@ class Transformer(nn.Module):
                 valid = pos_ < (torch.as_tensor(lens, device=arg.device)[:, None] - 1)
                 correct_list = [bool(v) for v in (ok | ~valid).all(1).tolist()]
         return probs_res, word_attention_map, correct_list
+
+    def beam_search(self, image, beams=4, max_len=60):
+        """the `beams` most likely stroke strings of every image: (tokens int64 [B, beams, max_len], log-probabilities fp32 [B,
+        beams]), best first, closed with '0' (fudanocr_amd/sld/beam.py).  image NCHW [B, 1 or 4, 32, 128]; eval mode."""
+        from ..sld import beam
+        with torch.no_grad():
+            if image.shape[1] == 4:
+                image = K.bicubic_gray(image, image.shape[3])
+            feat = self.encoder(image)
+        return beam.search(self, feat, self.embedding_word_with_upperword, self.generator_word_with_upperword, beams, max_len,
+                           alphabet.index("0"), alphabet.index("0"))

@@ -626,3 +626,84 @@ def test_search_steps_equal_dense_caches(dtype):
             dense[layer] = [dense[layer][s // beams * beams + int(parents.view(-1)[s])] for s in range(slots)]
     owned = torch.cat([cache.table.flatten(), cache.spare]).unique()
     assert owned.numel() >= slots                                     # no spare page was lost on the way
+
+
+# ---------------------------------------------------------------------------------------------- GPU: the recognizers
+def _recognizer(kind):
+    from fudanocr_amd.utils.weight_fill import fill_module_
+    if kind == "strokes":
+        from fudanocr_amd.sld.model.transformer import Transformer
+        m = Transformer("stroke")
+    elif kind == "characters":
+        from fudanocr_amd.loss.transformer import Transformer
+        m = Transformer()
+    else:
+        from fudanocr_amd.loss.transformer_english_decomposition import Transformer
+        m = Transformer()
+    fill_module_(m)
+    return m.cuda().eval()
+
+
+def _dense_logits(model, kind, image, tokens):
+    """[N, L, vocab] by the models' own forward on whole prefixes"""
+    with torch.no_grad():
+        if kind == "strokes":
+            length = torch.full((tokens.shape[0],), tokens.shape[1])
+            return model(image, length, tokens, test=True)["pred"]
+        return model.forward_padded(image, tokens)[0]
+
+
+@gpu
+@pytest.mark.parametrize("kind,channels,width", [("strokes", 3, 32), ("characters", 1, 128), ("english_strokes", 4, 128)])
+@pytest.mark.parametrize("beams", [1, 3])
+def test_recognizers_beam_search_equals_whole_prefixes(kind, channels, width, beams):
+    """the cached search against the same search by whole prefixes through the model's own forward and a 64-bit selection on
+    the CPU.  The two sum in another order, so scores agree to fp32 products over the network (1e-3 relative) and a hypothesis may
+    differ only where the dense search has one of the same score."""
+    model = _recognizer(kind)
+    g = torch.Generator().manual_seed(5)
+    batch, steps = 3, 20                                              # past a page of 16 tokens
+    image = (torch.rand(batch, channels, 32, width, generator=g) * 2 - 1).cuda()
+    tokens, scores = model.beam_search(image, beams=beams, max_len=steps)
+    assert tokens.shape == (batch, beams, steps) and scores.shape == (batch, beams)
+    assert (scores[:, :-1] >= scores[:, 1:]).all()
+    start, eos = (0, 6) if kind == "strokes" else (0, 0)
+    ended = (tokens == eos).int().cummax(-1).values.bool()
+    assert (tokens[ended] == eos).all()                               # nothing but eos behind the first one
+    # a hypothesis' score is the sum of its tokens' log-probabilities, by the dense forward
+    rep = image.repeat_interleave(beams, 0)
+    flat = tokens.view(-1, steps)
+    prefix = torch.cat([torch.full_like(flat[:, :1], start), flat[:, :-1]], 1)
+    logp = torch.log_softmax(_dense_logits(model, kind, rep, prefix).double(), -1)
+    per = torch.gather(logp, 2, flat[..., None])[..., 0]
+    live = torch.cat([torch.ones_like(ended.view(-1, steps)[:, :1]), ~ended.view(-1, steps)[:, :-1]], 1)
+    want = (per * live).sum(1).view(batch, beams)
+    ok = torch.isfinite(scores)
+    assert ok[:, 0].all() and ((scores.double() - want).abs() <= 1e-3 * (1 + want.abs()))[ok].all()
+    # the dense search, beam by beam
+    beam_scores = torch.full((batch, beams), float("-inf"), dtype=torch.float32)
+    beam_scores[:, 0] = 0
+    done = torch.zeros(batch, beams, dtype=torch.bool)
+    seqs = torch.full((batch, beams, 1), start)
+    for _ in range(steps):
+        lg = _dense_logits(model, kind, rep, seqs.view(batch * beams, -1).cuda())[:, -1].view(batch, beams, -1).cpu()
+        val, par, tok, fin = select_reference(lg, beam_scores, done, eos, beams)
+        seqs = torch.cat([torch.gather(seqs, 1, par.long()[..., None].expand(-1, -1, seqs.shape[2])), tok[..., None]], 2)
+        beam_scores, done = val.float(), fin
+    assert (beam_scores - scores.cpu()).abs().max() <= 1e-3 * (1 + beam_scores.abs().max())
+    for b in range(batch):
+        for j in range(beams):
+            if not torch.equal(seqs[b, j, 1:], tokens[b, j].cpu()):
+                close = (beam_scores[b] - scores[b, j].cpu()).abs() <= 2e-3 * (1 + scores[b, j].abs().item())
+                assert int(close.sum()) > 1, (b, j)
+
+
+@gpu
+def test_recognizer_beam_search_refusals():
+    model = _recognizer("strokes")
+    image = torch.zeros(1, 3, 32, 32).cuda()
+    _raises("1 to 64", model.beam_search, image, beams=0)
+    _raises("1 to 64", model.beam_search, image, beams=65)
+    _raises("max_len", model.beam_search, image, max_len=7001)
+    assert model.beam_search(image, beams=2, max_len=1)[0].shape == (1, 2, 1)
+    _raises("eval mode", model.train().beam_search, image)
