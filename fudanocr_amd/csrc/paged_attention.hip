@@ -9,6 +9,8 @@
 typedef _Float16 f16_t;
 typedef __bf16 bf16_t;
 
+typedef unsigned long long u64_mask;
+
 // the last i in [0, n) with f(i) <= key, for a non-decreasing f with f(0) <= key (64 probes a round; all lanes take part)
 template <typename F>
 __device__ __forceinline__ int pg_find(F f, int n, long key, int lane) {
@@ -150,6 +152,13 @@ __device__ __forceinline__ float pg_with_nonfinite(float x, float pos, float neg
   if (pos > 0.f) x += INFINITY;
   if (neg > 0.f) x -= INFINITY;
   return nan > 0.f ? NAN : x;
+}
+
+// exp2(c2 (s - mx)), ref = c2 mx (0 when there is no maximum yet).  One multiply-add; in fp32, where the matrix instructions
+// leave time, from the difference, which loses nothing near the maximum
+template <typename T> __device__ __forceinline__ float pg_weight(float s, float c2, float mx, float ref) {
+  if constexpr (sizeof(T) == 4) return __builtin_amdgcn_exp2f((s - (mx == -INFINITY ? 0.f : mx)) * c2);
+  else return __builtin_amdgcn_exp2f(fmaf(s, c2, -ref));
 }
 
 // a part's sum of weights relative to the common maximum; a part without keys has sum 0 at maximum -inf, one whose scores are
@@ -410,7 +419,7 @@ __global__ __launch_bounds__(256, (pg_thin_waves<T, D, NT>())) void paged_thin_k
       for (int sub = 0; sub < KT / 16; ++sub)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          p[sub * 4 + i] = __builtin_amdgcn_exp2f(fmaf(sc[t][sub][i], a.c2, -ref));
+          p[sub * 4 + i] = pg_weight<T>(sc[t][sub][i], a.c2, mx, ref);
           l[t] += p[sub * 4 + i];
         }
 #pragma unroll
@@ -566,20 +575,37 @@ __global__ __launch_bounds__(64 * NW, (pg_tile_waves<T, D, NW>())) void paged_ti
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l32 = lane & 31, hh = lane >> 5;
   const PagedShape& c = a.c;
   const long tiles = paged_tiles(c.tokens, c.seqs, a.group, ROWS);
-  const int kh = blockIdx.x % a.kv_heads;
-  const long ti = tiles - 1 - blockIdx.x / a.kv_heads % tiles;          // the tiles with the most keys first
-  const int split = (int)(blockIdx.x / a.kv_heads / tiles);
+  const int kh = blockIdx.x % a.kv_heads, split = (int)(blockIdx.x / a.kv_heads / tiles);
+  const long turn = blockIdx.x / a.kv_heads % tiles;
+  // The tiles with the most keys first, so that the last blocks to finish are short ones.  Up to 64 sequences are put in order of
+  // their lengths by the wave itself (24 chunks of 1 .. 764 tokens behind 300 .. 4000: 216 us in the order of the rows, 205 us
+  // so); more of them fill the card well enough from the last row to the first.
   int s;
-  if (c.q_start) {
-    const int* qs = c.q_start;
-    const int grp = a.group;
-    s = pg_find([=](int i) { return paged_first_tile(qs[i], i, grp, ROWS); }, c.seqs, ti, lane);
+  long tile;
+  if (c.seqs <= 64) {
+    int len = 0, mine = 0, start = 0;
+    if (lane < c.seqs) {
+      const PagedSeq sq = paged_seq(c, lane);
+      len = sq.len;
+      if ((long)sq.n * a.group > a.thin_rows) mine = (int)(((long)sq.n * a.group + ROWS - 1) / ROWS);
+    }
+    for (int j = 0; j < c.seqs; ++j) {
+      const int lj = __builtin_amdgcn_readlane(len, j), tj = __builtin_amdgcn_readlane(mine, j);
+      if (lj > len || (lj == len && j < lane)) start += tj;
+    }
+    const u64_mask hit = __ballot(turn >= start && turn < (long)start + mine);
+    if (!hit) return;
+    s = __builtin_ctzll(hit);
+    tile = __builtin_amdgcn_readlane(mine, s) - 1 - (turn - __builtin_amdgcn_readlane(start, s));
   } else {
-    const long n = c.tokens / c.seqs, grp = a.group;
-    s = pg_find([=](int i) { return paged_first_tile(i * n, i, (int)grp, ROWS); }, c.seqs, ti, lane);
+    const int* qs = c.q_start;
+    const long n = c.tokens / c.seqs, at = tiles - 1 - turn;
+    const int grp = a.group;
+    s = pg_find([=](int i) { return paged_first_tile(qs ? qs[i] : i * n, i, grp, ROWS); }, c.seqs, at, lane);
+    tile = at - paged_first_tile(qs ? qs[s] : s * n, s, grp, ROWS);
   }
   const PagedSeq sq = paged_seq(c, s);
-  const long R = (long)sq.n * a.group, r0 = (ti - paged_first_tile(sq.t0, s, a.group, ROWS)) * ROWS;
+  const long R = (long)sq.n * a.group, r0 = tile * ROWS;
   if (r0 < 0 || r0 >= R || R <= a.thin_rows) return;
   if (sq.bad || sq.n > a.max_q) {
     if (split == 0)
@@ -789,7 +815,7 @@ __global__ __launch_bounds__(64 * NW, (pg_tile_waves<T, D, NW>())) void paged_ti
       float p[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        p[i] = __builtin_amdgcn_exp2f(fmaf(sc[sub][i], a.c2, -ref));
+        p[i] = pg_weight<T>(sc[sub][i], a.c2, mx, ref);
         l += p[i];
       }
 #pragma unroll
@@ -1042,7 +1068,8 @@ extern "C" int focr_paged_attention_fwd(const void* q, long ldt, long ldh, const
   PG_CHECK_COMMON();
   FOCR_CHECK_ARG(q && o, "null pointer");
   FOCR_CHECK_ARG(kv_heads > 0 && heads > 0 && heads % kv_heads == 0, "heads must be a multiple of kv_heads");
-  FOCR_CHECK_ARG(max_q >= 0 && max_kv >= 0, "max_q / max_kv out of range");
+  FOCR_CHECK_ARG(max_q >= 0 && max_kv >= 0 && max_kv <= INT32_MAX - 16384, "max_q / max_kv out of range");
+  FOCR_CHECK_ARG(pg_aligned(ws), "workspace must be 16-byte aligned");
   FOCR_CHECK_ARG(scale > 0.f && scale < INFINITY, "scale must be positive and finite");
   FOCR_CHECK_ARG(q_start || tokens / seqs <= max_q, "max_q is below tokens / seqs");
   PagedShape c;

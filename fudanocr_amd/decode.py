@@ -2,8 +2,8 @@
 of new tokens over it, beam search's selection and the reordering of the surviving beams' caches.
 
 The recognizers' `beam_search` (fudanocr_amd/sld/beam.py) is built from these; they work on their own as well.  Unlike the
-training operators of `kernels` / `sld.ops` they also take bf16 and fp16 tensors, keep no graph, and nothing in them waits
-for the device: lengths, tables and parents stay there.
+training operators of `kernels` / `sld.ops` they also take bf16 and fp16 tensors, have no backward pass (a tensor that wants a
+gradient is refused), and nothing in them waits for the device: lengths, tables and parents stay there.
 
 A cache is four tensors:
 
@@ -28,6 +28,8 @@ from .kernels import _RAW_STREAM
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _PAGES, _DIMS = frozenset(8 << i for i in range(8)), (64, 128, 256)
+_LONGEST = 2 ** 31 - 2 ** 14 - 1          # tokens of a sequence: positions and the steps beyond the last one are 32-bit numbers
+_NO_GRAD = "%s wants a gradient, which these operators do not have (torch.no_grad(), or kernels / sld.ops in training)"
 _EVEN = "without q_start every sequence has the same number of rows; %d tokens, %d sequences"
 
 
@@ -89,6 +91,7 @@ def _rows(t, heads, dim, dt, dev, what):
           "heads" if heads is None else heads, dim, dt)
     st = t.stride()
     _need(st[2] == 1 or t.numel() == 0, "%s must have contiguous rows of dim", what)
+    _need(not t.requires_grad or not torch.is_grad_enabled(), _NO_GRAD, what)
     return st[0], st[1]
 
 
@@ -123,16 +126,16 @@ def paged_attention(q, k_pages, v_pages, table, kv_lens, q_start=None, causal=Tr
     _need(q_start is not None or seqs == 0 or tokens % seqs == 0, _EVEN, tokens, seqs)
     scale = dim ** -0.5 if scale is None else float(scale)
     _need(0.0 < scale < math.inf, "scale must be positive and finite, got %r", scale)
-    limit = ld * page
+    limit = min(ld * page, _LONGEST)
     max_kv = limit if max_kv is None else min(int(max_kv), limit)
     if q_start is None:
         max_q = tokens // seqs if seqs else 0
     else:
         max_q = tokens if max_q is None else min(int(max_q), tokens)
-    _need(max_q >= 0 and 0 <= max_kv < 2 ** 31, "max_q / max_kv out of range")
+    _need(max_q >= 0 and max_kv >= 0, "max_q / max_kv out of range")
     if out is not None:
         os = _rows(out, heads, dim, dt, dev, "out")
-        _need(out.shape[0] == tokens, "out must have q's shape")
+        _need(out.shape[0] == tokens and os[0] != 0 and os[1] != 0, "out must have q's shape and rows of its own")
         _need(not _overlap(out, q), "out must not share q's memory")
     _on_gpu(k_pages)
     if out is None:
@@ -176,6 +179,7 @@ def beam_select(logits, scores, finished=None, eos=None, n=None):
           "beams and n must be 1 to 64 and n at most beams * vocab; got %d beams, n = %d, vocab %d", beams, n, vocab)
     ls = logits.stride()
     _need(ls[2] == 1 or vocab == 1 or logits.numel() == 0, "logits must have contiguous rows of vocab")
+    _need(not logits.requires_grad or not torch.is_grad_enabled(), _NO_GRAD, "logits")
     _need(scores.dtype is torch.float32 and scores.shape == (batch, beams) and scores.is_contiguous()
           and scores.get_device() == dev, "scores must be a contiguous fp32 tensor [batch, beams] on the logits' device")
     if finished is not None:

@@ -144,6 +144,11 @@ def test_attention_refuses_bad_arguments():
     for scale in (0.0, -1.0, math.inf, math.nan):
         _raises("scale", D.paged_attention, q, *c, scale=scale)
     _raises("out must have q's shape", D.paged_attention, q, *c, out=torch.zeros(4, 4, 64))
+    _raises("rows of its own", D.paged_attention, q, *c, out=torch.zeros(1, 4, 64).expand(3, 4, 64))
+    _raises("wants a gradient", D.paged_attention, q.clone().requires_grad_(True), *c)
+    _raises("wants a gradient", D.paged_append, torch.zeros(3, 2, 64, requires_grad=True), torch.zeros(3, 2, 64), *c)
+    with torch.no_grad():
+        _raises("on the GPU", D.paged_attention, q.clone().requires_grad_(True), *c)
     _raises("share q's memory", D.paged_attention, q, *c, out=q)
     _raises("k_new must be", D.paged_append, q, q, *c)
     _raises("same tokens", D.paged_append, torch.zeros(3, 2, 64), torch.zeros(6, 2, 64), *c)
@@ -154,6 +159,7 @@ def test_beam_operators_refuse_bad_arguments():
     _raises("on the GPU", D.beam_select, x, s)
     _raises("logits must be", D.beam_select, x.double(), s)
     _raises("logits must be", D.beam_select, x[0], s)
+    _raises("wants a gradient", D.beam_select, x.clone().requires_grad_(True), s)
     _raises("1 to 64", D.beam_select, torch.zeros(1, 65, 7), torch.zeros(1, 65))
     _raises("n at most", D.beam_select, torch.zeros(1, 2, 3), torch.zeros(1, 2), n=7)
     _raises("contiguous rows", D.beam_select, torch.zeros(2, 7, 3).transpose(1, 2), s)
@@ -188,7 +194,7 @@ def test_c_entries_refuse_before_they_launch():
         return lib.focr_paged_attention_fwd(*a.values(), None), lib.focr_last_error().decode()
     for kw, text in ((dict(dt=3), "dtype"), (dict(dim=65), "head dim"), (dict(page=24), "power of two"), (dict(page=2048), "power of two"),
                      (dict(k=p + 8), "aligned"), (dict(o=None), "null"), (dict(heads=3), "multiple"), (dict(pages=0), "empty"),
-                     (dict(tokens=4), "tokens / seqs"), (dict(tokens=6), "max_q"), (dict(scale=0.0), "scale"), (dict(tokens=-1), "range")):
+                     (dict(ws=p + 4), "aligned"), (dict(max_kv=2 ** 31 - 1), "max_kv"), (dict(tokens=4), "tokens / seqs"), (dict(tokens=6), "max_q"), (dict(scale=0.0), "scale"), (dict(tokens=-1), "range")):
         rc, msg = call(**kw)
         assert rc == -1 and text in msg, (kw, rc, msg)
     assert call(tokens=0)[0] == 0 and call(seqs=0)[0] == 0
@@ -237,6 +243,45 @@ def test_attention_splits_long_caches(dtype, page, n, length, heads, kv_heads):
     pool = Pool([length, length // 3], kv_heads, 128, page, dtype, seed=page)
     q = (2 * torch.randn(2 * n, heads, 128, generator=torch.Generator().manual_seed(1))).to(dtype)
     ref, tol = reference(q, pool.dense, [0, n], [n, n], True, 128 ** -0.5)
+    check(D.paged_attention(q.cuda(), *pool.args), ref, tol)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("heads", [20, 33, 71])
+def test_many_heads_on_one_key_head(dtype, heads):
+    """groups of no even size, up to more rows in one token than the thin kernel takes"""
+    news, lens = [1, 3, 1, 0, 6], [40, 3, 700, 9, 129]
+    pool = Pool(lens, 1, 128, 32, dtype)
+    starts = starts_of(news)
+    q = (2 * torch.randn(starts[-1], heads, 128, generator=torch.Generator().manual_seed(1))).to(dtype)
+    ref, tol = reference(q, pool.dense, starts, news, True, 128 ** -0.5)
+    qs = torch.tensor(starts, dtype=torch.int32).cuda()
+    check(D.paged_attention(q.cuda(), *pool.args, q_start=qs), ref, tol)
+    check(D.paged_attention(q.cuda(), *pool.args, q_start=qs, max_q=6, max_kv=700), ref, tol)
+    one = q[:5]
+    ref, tol = reference(one, pool.dense, list(range(5)), [1] * 5, True, 128 ** -0.5)
+    check(D.paged_attention(one.cuda(), *pool.args), ref, tol)
+
+
+@gpu
+@pytest.mark.parametrize("seqs", [64, 65, 150])
+@pytest.mark.parametrize("long_ones", [3, 60])
+def test_many_sequences_of_mixed_lengths(seqs, long_ones):
+    """single tokens, empty ones and chunks side by side, more sequences than a wave has lanes; few long ones (both kernels, a
+    launch each) and many (the tiles take the single tokens along)"""
+    rng = random.Random(seqs)
+    news = [rng.choice([0, 1, 1, 1, 2]) for _ in range(seqs)]
+    for i in rng.sample(range(seqs), long_ones):
+        news[i] = rng.randint(20, 90)
+    lens = [n + rng.choice([0, 5, 33, 200]) for n in news]
+    pool = Pool(lens, 2, 64, 16, torch.bfloat16)
+    starts = starts_of(news)
+    q = torch.randn(starts[-1], 8, 64, generator=torch.Generator().manual_seed(1)).bfloat16()
+    ref, tol = reference(q, pool.dense, starts, news, True, 0.125)
+    check(D.paged_attention(q.cuda(), *pool.args, q_start=torch.tensor(starts, dtype=torch.int32).cuda()), ref, tol)
+    q = torch.randn(9 * seqs, 8, 64, generator=torch.Generator().manual_seed(2)).bfloat16()
+    ref, tol = reference(q, pool.dense, [9 * i for i in range(seqs)], [9] * seqs, True, 0.125)
     check(D.paged_attention(q.cuda(), *pool.args), ref, tol)
 
 
