@@ -27,7 +27,7 @@ __device__ __forceinline__ int pg_find(F f, int n, long key, int lane) {
 }
 
 __device__ __forceinline__ int pg_seq_of_row(const PagedShape& c, long t, int lane) {
-  if (!c.q_start) return (int)(t / (c.tokens / c.seqs));
+  if (!c.q_start) return (int)t / c.per;
   const int* q = c.q_start;
   return pg_find([q](int i) { return q[i]; }, c.seqs, t, lane);
 }
@@ -177,7 +177,7 @@ struct PgArgs {
   long ldto, ldho;
   float* part;   // [split][token][head][D], weights relative to the split's own maximum
   float2* ml;    // [split][token][head]: that maximum (in log2 units) and the sum of the weights
-  int max_q, heads, kv_heads, group, nsplit, chunk, tile_chunk, causal, thin_rows, wide_q, wide_o;
+  int max_q, heads, kv_heads, group, nsplit, chunk, tile_chunk, tiles, causal, thin_rows, wide_q, wide_o;
   float c2;      // scale * log2(e)
 };
 
@@ -259,7 +259,7 @@ __global__ __launch_bounds__(256, (pg_thin_waves<T, D, NT>())) void paged_thin_k
   // splits in the slowest place: blocks go round the 8 XCDs by number, and the last splits of most sequences are empty
   const int kh = blockIdx.x % a.kv_heads, s = blockIdx.x / a.kv_heads % c.seqs, split = blockIdx.x / a.kv_heads / c.seqs;
   const PagedSeq sq = paged_seq(c, s);
-  if ((long)sq.n * a.group > a.thin_rows && sq.n <= a.max_q) return;     // the other kernel's
+  if (sq.n * a.group > a.thin_rows && sq.n <= a.max_q) return;           // the other kernel's
   if (sq.n == 0) return;
   if (sq.bad || sq.n > a.max_q) {
     if (split == 0 && (sq.n <= a.max_q || a.thin_rows >= a.max_q * a.group)) pg_fill_nan<T, D>(a, sq, kh, 256);
@@ -574,48 +574,46 @@ __global__ __launch_bounds__(64 * NW, (pg_tile_waves<T, D, NW>())) void paged_ti
   char* const vsm = pg_smem + 2 * KT * ROWB;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l32 = lane & 31, hh = lane >> 5;
   const PagedShape& c = a.c;
-  const long tiles = paged_tiles(c.tokens, c.seqs, a.group, ROWS);
-  const int kh = blockIdx.x % a.kv_heads, split = (int)(blockIdx.x / a.kv_heads / tiles);
-  const long turn = blockIdx.x / a.kv_heads % tiles;
+  const int kh = blockIdx.x % a.kv_heads, split = blockIdx.x / a.kv_heads / a.tiles;
+  const int turn = blockIdx.x / a.kv_heads % a.tiles;
   // The tiles with the most keys first, so that the last blocks to finish are short ones.  Up to 64 sequences are put in order of
   // their lengths by the wave itself (24 chunks of 1 .. 764 tokens behind 300 .. 4000: 216 us in the order of the rows, 205 us
   // so); more of them fill the card well enough from the last row to the first.
-  int s;
-  long tile;
+  int s, tile;
   if (c.seqs <= 64) {
     int len = 0, mine = 0, start = 0;
     if (lane < c.seqs) {
       const PagedSeq sq = paged_seq(c, lane);
       len = sq.len;
-      if ((long)sq.n * a.group > a.thin_rows) mine = (int)(((long)sq.n * a.group + ROWS - 1) / ROWS);
+      if (sq.n * a.group > a.thin_rows) mine = (sq.n * a.group + ROWS - 1) / ROWS;
     }
     for (int j = 0; j < c.seqs; ++j) {
       const int lj = __builtin_amdgcn_readlane(len, j), tj = __builtin_amdgcn_readlane(mine, j);
       if (lj > len || (lj == len && j < lane)) start += tj;
     }
-    const u64_mask hit = __ballot(turn >= start && turn < (long)start + mine);
+    const u64_mask hit = __ballot(turn >= start && turn - start < mine);
     if (!hit) return;
     s = __builtin_ctzll(hit);
     tile = __builtin_amdgcn_readlane(mine, s) - 1 - (turn - __builtin_amdgcn_readlane(start, s));
   } else {
     const int* qs = c.q_start;
-    const long n = c.tokens / c.seqs, at = tiles - 1 - turn;
+    const long n = c.per, at = a.tiles - 1 - turn;
     const int grp = a.group;
     s = pg_find([=](int i) { return paged_first_tile(qs ? qs[i] : i * n, i, grp, ROWS); }, c.seqs, at, lane);
-    tile = at - paged_first_tile(qs ? qs[s] : s * n, s, grp, ROWS);
+    tile = (int)(at - paged_first_tile(qs ? qs[s] : s * n, s, grp, ROWS));
   }
   const PagedSeq sq = paged_seq(c, s);
-  const long R = (long)sq.n * a.group, r0 = tile * ROWS;
-  if (r0 < 0 || r0 >= R || R <= a.thin_rows) return;
+  const int R = sq.n * a.group, r0 = tile * ROWS;      // (the host has checked that tokens x heads and a tile more fit)
+  if (tile < 0 || r0 >= R || R <= a.thin_rows) return;
   if (sq.bad || sq.n > a.max_q) {
     if (split == 0)
-      for (long x = tid; x < ROWS * D; x += 64 * NW) {
-        const long r = r0 + x / D;
+      for (int x = tid; x < ROWS * D; x += 64 * NW) {
+        const int r = r0 + x / D;
         if (r < R) a.o[(sq.t0 + r / a.group) * a.ldto + (kh * a.group + r % a.group) * a.ldho + x % D] = (T)NAN;
       }
     return;
   }
-  const int tok0 = (int)(r0 / a.group), tok1 = (int)((R < r0 + ROWS ? R - 1 : r0 + ROWS - 1) / a.group);
+  const int tok0 = r0 / a.group, tok1 = (R < r0 + ROWS ? R - 1 : r0 + ROWS - 1) / a.group;
   const int vmin = paged_visible(sq.len, sq.n, tok0, a.causal), kend = paged_visible(sq.len, sq.n, tok1, a.causal);
   const bool direct = sq.len <= a.tile_chunk;
   const int k0 = split * a.tile_chunk;
@@ -625,11 +623,10 @@ __global__ __launch_bounds__(64 * NW, (pg_tile_waves<T, D, NW>())) void paged_ti
 
   // this wave's rows: one query column per lane
   u32x4 qf[NU];
-  const long row = r0 + wave * 32 + l32;
+  const int row = r0 + wave * 32 + l32;
   const bool ok = row < R;
-  const long tok = ok ? row / a.group : 0;
-  const int head = kh * a.group + (ok ? (int)(row - tok * a.group) : 0);
-  const int vis = ok ? paged_visible(sq.len, sq.n, (int)tok, a.causal) : 0;
+  const int tok = ok ? row / a.group : 0, head = kh * a.group + (ok ? row - tok * a.group : 0);
+  const int vis = ok ? paged_visible(sq.len, sq.n, tok, a.causal) : 0;
   int wvmin = ok ? vis : INT32_MAX, wvmax = vis;
   const T* p = a.q + (sq.t0 + tok) * a.ldt + head * a.ldh + hh * EC;
 #pragma unroll
@@ -865,13 +862,13 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PgArgs<T> a) {
   constexpr int E = D / 64;
   __shared__ float wmax[4], wsum[4], acc[3][D];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = wave % WPR;
-  const long row = (long)blockIdx.x * (4 / WPR) + wave / WPR, rows = a.c.tokens * a.heads;
+  const long rows = a.c.tokens * a.heads;
+  const int row = blockIdx.x * (4 / WPR) + wave / WPR;
   if (row >= rows) return;                             // (with 4 waves a row there is no such row)
-  const long t = row / a.heads;
-  const int h = (int)(row - t * a.heads), s = pg_seq_of_row(a.c, t, lane);
+  const int t = row / a.heads, h = row - t * a.heads, s = pg_seq_of_row(a.c, t, lane);
   const PagedSeq sq = paged_seq(a.c, s);
   const long i = t - sq.t0;
-  const int chunk = (long)sq.n * a.group <= a.thin_rows ? a.chunk : a.tile_chunk;
+  const int chunk = sq.n * a.group <= a.thin_rows ? a.chunk : a.tile_chunk;
   if (i < 0 || i >= sq.n || sq.bad || sq.n > a.max_q || sq.len <= chunk) return;
   const int n = (paged_visible(sq.len, sq.n, (int)i, a.causal) + chunk - 1) / chunk;
   float mx = -INFINITY;
@@ -913,7 +910,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PgArgs<T> a) {
 static bool pg_shape(PagedShape& c, const int* table, const int* kv_lens, const int* q_start, long tokens, int seqs, int page,
                      int table_ld, long num_pages, int max_kv) {
   if (page < 8 || page > 1024 || (page & (page - 1))) return false;
-  c = {table, kv_lens, q_start, tokens, num_pages, seqs, table_ld, __builtin_ctz(page), max_kv};
+  c = {table, kv_lens, q_start, tokens, num_pages, seqs, table_ld, __builtin_ctz(page), max_kv, q_start ? 0 : (int)(tokens / seqs)};
   return true;
 }
 static bool pg_aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -1043,8 +1040,9 @@ static int pg_run(PgArgs<T> a, long ws_bytes, hipStream_t st) {
     a.ml = (float2*)(a.part + need / ((D + 2) * 4) * D);
   }
   const long thin = (long)p.nsplit * a.kv_heads * c.seqs;
-  const long tiles = paged_tiles(c.tokens, c.seqs, a.group, 32 * p.tile_waves) * a.kv_heads * p.tsplit;
-  if (thin > INT32_MAX || tiles > INT32_MAX || rows > INT32_MAX) return FOCR_EUNSUPPORTED;
+  const long per_head = paged_tiles(c.tokens, c.seqs, a.group, 32 * p.tile_waves), tiles = per_head * a.kv_heads * p.tsplit;
+  if (thin > INT32_MAX || tiles > INT32_MAX || rows > INT32_MAX - 4096) return FOCR_EUNSUPPORTED;
+  a.tiles = (int)per_head;
   if ((long)a.max_q * a.group > 32) {
     int rc;
     if constexpr (WIDE) rc = p.tile_waves == 8 ? pg_launch_tiles<T, D, 8>(a, tiles, st) : pg_launch_tiles<T, D, 4>(a, tiles, st);
@@ -1080,7 +1078,7 @@ extern "C" int focr_paged_attention_fwd(const void* q, long ldt, long ldh, const
   const bool wo = pg_aligned(o) && (((ldto | ldho) * pg_esize(dtype)) & 15) == 0;
 #define PG_RUN(T, DD)                                                                                                       \
   rc = pg_run<T, DD>(PgArgs<T>{(const T*)q, ldt, ldh, (const T*)k_pages, (const T*)v_pages, c, (T*)o, ldto, ldho, (float*)ws, \
-                               nullptr, max_q, heads, kv_heads, heads / kv_heads, 1, 0, 0, causal ? 1 : 0, 0, wq, wo,             \
+                               nullptr, max_q, heads, kv_heads, heads / kv_heads, 1, 0, 0, 0, causal ? 1 : 0, 0, wq, wo,             \
                                scale * 1.4426950408889634f}, ws_bytes, (hipStream_t)stream)
 #define PG_RUN_D(T)                    \
   if (dim == 64) PG_RUN(T, 64);        \

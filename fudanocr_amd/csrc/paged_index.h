@@ -14,9 +14,10 @@
 struct PagedShape {
   const int* table;    // [seqs][table_ld]
   const int* kv_lens;  // [seqs]
-  const int* q_start;  // [seqs + 1] first row of each sequence's new tokens, or null: tokens / seqs rows each
+  const int* q_start;  // [seqs + 1] first row of each sequence's new tokens, or null: `per` rows each
   long tokens, num_pages;
   int seqs, table_ld, page_shift, max_kv;
+  int per;             // tokens / seqs where there is no q_start (a 64-bit division is not for every block to do)
 };
 
 struct PagedSeq {
@@ -35,7 +36,7 @@ PG_FN PagedSeq paged_seq(const PagedShape& c, int s) {
     r.t0 = ok ? a : 0;
     r.n = ok ? (int)(b - a) : 0;
   } else {
-    r.n = (int)(c.tokens / c.seqs);
+    r.n = c.per;
     r.t0 = (long)s * r.n;
   }
   const int len = c.kv_lens[s];

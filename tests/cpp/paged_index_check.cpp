@@ -32,6 +32,7 @@ int main() {
     if (spoilt) qs[pick(0, c.seqs)] = junk[pick(0, 4)];
     c.table = table.data(); c.kv_lens = lens.data(); c.q_start = qs.data();
     if (pick(0, 3) == 0) { c.q_start = nullptr; c.tokens = c.seqs * pick(0, 70); }
+    c.per = c.q_start ? 0 : (int)(c.tokens / c.seqs);
     for (int s = 0; s < c.seqs; ++s) {
       const PagedSeq q = paged_seq(c, s);
       REQUIRE(q.n >= 0 && q.t0 >= 0 && q.t0 + q.n <= c.tokens);
