@@ -954,12 +954,15 @@ extern "C" int focr_paged_append(const void* k_new, const void* v_new, long ldtk
 // blocks 198 us, 4096 193 us, 8192 200 us), but no fewer than 1024 keys in a block while there are blocks enough for two on each
 // CU: a block's start and end cost as much as some hundred keys (2 sequences of 131k: 1024 keys 205 us, 512 224 us, 256 254 us).
 //
-// Calls with longer chunks go to the tile kernel: 128 rows a block, and split over keys only when there are fewer than two such
-// blocks a CU (24 chunks of 1 .. 764 tokens x 32 heads, bf16: 221 us unsplit, 232 / 240 us cut for 1024 / 2048 blocks: the parts
-// are written and read in fp32).  256 rows a block halve the reads from LDS per product, but make one block a CU: taken when
-// 128-row blocks would fill the card twice over and sequences are long (4096 tokens after 12288: 1058 -> 948 us; the 24 chunks:
-// 221 -> 250 us).  In a ragged call that has mostly short sequences those go to the thin kernel in a launch of their own; with
-// 32 rows a sequence or more on average the tiles take them along (the 24 chunks, 11 of them single tokens: 303 -> 221 us).
+// Calls with longer chunks go to the tile kernel, 128 rows a block.
+//   * Split over keys only when there are fewer than two such blocks a CU (24 chunks of 1 .. 764 tokens x 32 heads, bf16, 85 tiles x
+//     8 key heads: 221 us unsplit, 232 / 240 us cut for 1024 / 2048 blocks: the parts are written and read in fp32), into 1024 keys
+//     or more (1024 tokens alone, 32 heads: 37 us, in halves 48), fewer only when that leaves half of the CUs idle (4 chunks of 64
+//     behind 1000, fp32: 54 us, in halves 85).
+//   * 256 rows a block halve the reads from LDS per product, but make one block a CU: taken when 128-row blocks would fill the
+//     card twice over and sequences are long (4096 tokens after 12288: 1058 -> 948 us; the 24 chunks: 221 -> 250 us).
+//   * In a ragged call that has mostly short sequences those go to the thin kernel in a launch of their own; with 32 rows a
+//     sequence or more on average the tiles take them along (the 24 chunks, 11 of them single tokens: 303 -> 221 us).
 struct PgPlan {
   int thin_rows;           // sequences of at most this many rows go to the thin kernel, the rest to the tiles
   int nsplit, chunk;       // of the thin kernel
@@ -989,9 +992,13 @@ static PgPlan pg_plan(long tokens, int seqs, int kv_heads, int group, int max_q,
     const long blocks = (tokens * group + 127) / 128 * kv_heads;
     if (blocks < 512 && max_kv > 512) {
       long chunk = max_kv * blocks / 512;
-      chunk = ((chunk < 512 ? 512 : chunk) + 127) / 128 * 128;
-      p.tsplit = (int)((max_kv + chunk - 1) / chunk);
-      p.tile_chunk = (int)chunk;
+      if (chunk < 1024) chunk = 1024;
+      if (blocks * ((max_kv + chunk - 1) / chunk) < 256) chunk = max_kv * blocks / 256;
+      if (chunk < 256) chunk = 256;
+      if (chunk < max_kv) {
+        p.tsplit = (int)((max_kv + chunk - 1) / chunk);
+        p.tile_chunk = (int)(((max_kv + p.tsplit - 1) / p.tsplit + 127) / 128 * 128);
+      }
     }
     if (blocks >= 1024 && tokens * group >= 1024l * seqs) p.tile_waves = 8;
   }
