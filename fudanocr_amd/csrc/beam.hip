@@ -397,7 +397,7 @@ extern "C" int focr_beam_select(const void* logits, long ldb, long ldk, const fl
   FOCR_CHECK_ARG(logits && scores && out_scores && out_parents && out_tokens && out_finished, "null pointer");
   const BsPlan p = bs_plan(batch, beams, vocab);
   const long rows = (long)batch * beams * p.parts;
-  FOCR_CHECK_ARG(rows <= INT32_MAX - 4, "too many rows for one launch");
+  FOCR_CHECK_ARG(rows >> 26 == 0 && batch >> 22 == 0, "too many rows for one launch");
   FOCR_CHECK_ARG(p.one || (ws && ((uintptr_t)ws & 7) == 0 && ws_bytes >= focr_beam_select_ws_bytes(batch, beams, vocab, n, dtype)),
                  "workspace missing or too small (focr_beam_select_ws_bytes)");
   BsArgs a = {logits, ldb, ldk, scores, finished, out_scores, out_parents, out_tokens, out_finished, (u64_t*)ws,

@@ -156,10 +156,11 @@ __device__ __forceinline__ float pg_with_nonfinite(float x, float pos, float neg
 }
 
 // exp2(c2 (s - mx)), ref = c2 mx (0 when there is no maximum yet).  One multiply-add; in fp32, where the matrix instructions
-// leave time, from the difference, which loses nothing near the maximum
+// leave time, from the difference, which loses nothing near the maximum.  fp16 weights are taken 2^14 times as large, sums and all:
+// a long tail of weights below fp16's 6e-8 would count in the sum (fp32) and not in the product
 template <typename T> __device__ __forceinline__ float pg_weight(float s, float c2, float mx, float ref) {
   if constexpr (sizeof(T) == 4) return __builtin_amdgcn_exp2f((s - (mx == -INFINITY ? 0.f : mx)) * c2);
-  else return __builtin_amdgcn_exp2f(fmaf(s, c2, -ref));
+  else return __builtin_amdgcn_exp2f(fmaf(s, c2, (PgMma<T>::EXP == 0x7c00u ? 14.f : 0.f) - ref));
 }
 
 // a part's sum of weights relative to the common maximum; a part without keys has sum 0 at maximum -inf, one whose scores are
@@ -941,6 +942,7 @@ extern "C" int focr_paged_append(const void* k_new, const void* v_new, long ldtk
                                  int heads, int dim, int page, int table_ld, long num_pages, int dtype, void* stream) {
   PG_CHECK_COMMON();
   FOCR_CHECK_ARG(k_new && v_new && heads > 0, "null pointer or no heads");
+  FOCR_CHECK_ARG(tokens >> 26 == 0, "too many tokens for one launch");
   PagedShape c;
   FOCR_CHECK_ARG(pg_shape(c, table, kv_lens, q_start, tokens, seqs, page, table_ld, num_pages, INT32_MAX),
                  "page must be a power of two from 8 to 1024");
@@ -1058,7 +1060,8 @@ static int pg_run(PgArgs<T> a, long ws_bytes, hipStream_t st) {
   }
   const long thin = (long)p.nsplit * a.kv_heads * c.seqs;
   const long per_head = paged_tiles(c.tokens, c.seqs, a.group, 32 * p.tile_waves), tiles = per_head * a.kv_heads * p.tsplit;
-  if (thin > INT32_MAX || tiles > INT32_MAX || rows > INT32_MAX - 4096) return FOCR_EUNSUPPORTED;
+  // a launch has at most 2^32 threads in a direction
+  if (thin >> 24 || tiles >> 23 || rows > INT32_MAX - 4096 || (need && rows >> 26)) return FOCR_EUNSUPPORTED;
   a.tiles = (int)per_head;
   if ((long)a.max_q * a.group > 32) {
     int rc;
@@ -1069,7 +1072,7 @@ static int pg_run(PgArgs<T> a, long ws_bytes, hipStream_t st) {
   if (p.thin_rows > 16) hipLaunchKernelGGL((paged_thin_kernel<T, D, 2>), dim3((unsigned)thin), dim3(256), 0, st, a);
   else if (p.thin_rows) hipLaunchKernelGGL((paged_thin_kernel<T, D, 1>), dim3((unsigned)thin), dim3(256), 0, st, a);
   if (need) {
-    if (p.nsplit > 16 || p.tsplit > 16) hipLaunchKernelGGL((paged_join_kernel<T, D, 4>), dim3((unsigned)rows), dim3(256), 0, st, a);
+    if ((p.nsplit > 16 || p.tsplit > 16) && rows >> 24 == 0) hipLaunchKernelGGL((paged_join_kernel<T, D, 4>), dim3((unsigned)rows), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((paged_join_kernel<T, D, 1>), dim3(cdiv(rows, 4)), dim3(256), 0, st, a);
   }
   return FOCR_OK;

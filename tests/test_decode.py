@@ -248,6 +248,61 @@ def test_attention_splits_long_caches(dtype, page, n, length, heads, kv_heads):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("n,heads,kv_heads", [(3, 16, 2), (8, 8, 2), (1, 32, 1)])
+def test_rows_for_two_column_tiles(dtype, dim, n, heads, kv_heads):
+    """17 to 32 rows a key head, lengths around the tiles' and the waves' turns"""
+    lens = [n, 15, 16, 33, 64, 65, 127, 129, 300]
+    pool = Pool([max(n, x) for x in lens], kv_heads, dim, 8, dtype)
+    lens = pool.lens.tolist()
+    q = (2 * torch.randn(n * len(lens), heads, dim, generator=torch.Generator().manual_seed(1))).to(dtype)
+    for causal in (True, False):
+        ref, tol = reference(q, pool.dense, [i * n for i in range(len(lens))], [n] * len(lens), causal, dim ** -0.5)
+        check(D.paged_attention(q.cuda(), *pool.args, causal=causal), ref, tol)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_chunks_that_fill_the_card(dtype, dim):
+    """enough long chunks for 256-row tiles; 24 tokens of each, the first and the last among them, against 64 bits"""
+    news, lens, heads, kv_heads = [1100, 1301], [1500, 1301], 64, 64
+    pool = Pool(lens, kv_heads, dim, 64, dtype)
+    starts = starts_of(news)
+    g = torch.Generator().manual_seed(3)
+    q = (2 * torch.randn(starts[-1], heads, dim, generator=g)).to(dtype)
+    out = D.paged_attention(q.cuda(), *pool.args, q_start=torch.tensor(starts, dtype=torch.int32).cuda()).cpu()
+    for s in range(2):
+        for i in [0, news[s] - 1] + torch.randint(0, news[s], (22,), generator=g).tolist():
+            k, v = pool.dense[s][:, :lens[s] - news[s] + 1 + i]
+            ref, tol = reference(q[starts[s] + i][None], [(k, v)], [0], [1], True, dim ** -0.5)
+            check(out[starts[s] + i][None], ref, tol)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("n", [1, 40])
+def test_a_long_tail_of_small_weights_counts(dtype, n):
+    """one key that outweighs every other by e^17 and 60 000 others: together 0.25 % of the weight, each of them below the
+    smallest number fp16 has"""
+    length, dim = 60000, 64
+    pool = Pool([length], 1, dim, 64, dtype)
+    k, v = torch.zeros(length, 1, dim), torch.ones(length, 1, dim)
+    k[7, 0, 0], v[7] = 17.0, 0.0
+    for j in range(-(-length // 64)):
+        pg, rows = int(pool.table[0, j]), slice(j * 64, min(length, j * 64 + 64))
+        m = rows.stop - rows.start
+        pool.k[pg, :, :m], pool.v[pg, :, :m] = k[rows].transpose(0, 1).to(dtype).cuda(), v[rows].transpose(0, 1).to(dtype).cuda()
+    q = torch.zeros(n, 1, dim)
+    q[:, 0, 0] = 1.0
+    q = q.to(dtype)
+    ref, tol = reference(q, [(k.double(), v.double())], [0], [n], True, 1.0)
+    assert 0.002 < ref.max() < 0.003
+    check(D.paged_attention(q.cuda(), *pool.args, scale=1.0), ref, tol)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=["fp32", "bf16", "fp16"])
 @pytest.mark.parametrize("heads", [20, 33, 71])
 def test_many_heads_on_one_key_head(dtype, heads):
     """groups of no even size, up to more rows in one token than the thin kernel takes"""
