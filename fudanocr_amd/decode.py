@@ -26,6 +26,7 @@ import torch
 from . import _lib
 from .kernels import _RAW_STREAM
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _PAGES, _DIMS = frozenset(8 << i for i in range(8)), (64, 128, 256)
 _LONGEST = 2 ** 31 - 2 ** 14 - 1          # tokens of a sequence: positions and the steps beyond the last one are 32-bit numbers
@@ -40,7 +41,7 @@ def _need(ok, what, *args):
 
 def _launch(device, name, *args):
     """the entry point on the current stream of the tensors' device (an index), whatever device is current"""
-    if device == torch.cuda.current_device():
+    if device == _current_device():
         _lib.call(name, *args, _stream(device))
     else:
         with torch.cuda.device(device):
@@ -65,6 +66,16 @@ def _int32(t, shape, dev, what):
 
 def _cache(k_pages, v_pages, table, kv_lens, q_start):
     shape, dt, dev = k_pages.shape, k_pages.dtype, k_pages.get_device()
+    tshape = table.shape
+    # all of it in one condition (a call per check takes longer than the kernel of a small step); what is wrong is said below
+    if (len(shape) == 4 and shape == v_pages.shape and dt is v_pages.dtype and dt in _DTYPES and k_pages.is_contiguous()
+            and v_pages.is_contiguous() and v_pages.get_device() == dev and shape[2] in _PAGES and shape[3] in _DIMS
+            and shape[0] > 0 and shape[1] > 0 and len(tshape) == 2 and tshape[1] > 0 and table.dtype is torch.int32
+            and table.is_contiguous() and table.get_device() == dev and kv_lens.dtype is torch.int32
+            and kv_lens.shape == (tshape[0],) and kv_lens.is_contiguous() and kv_lens.get_device() == dev
+            and (q_start is None or (q_start.dtype is torch.int32 and q_start.shape == (tshape[0] + 1,)
+                                     and q_start.is_contiguous() and q_start.get_device() == dev))):
+        return *shape, *tshape, dt, dev
     _need(len(shape) == 4 and shape == v_pages.shape and dt is v_pages.dtype and dt in _DTYPES,
           "k_pages and v_pages must be two [num_pages, heads, page, dim] tensors of one type (fp32, bf16 or fp16)")
     _need(k_pages.is_contiguous() and v_pages.is_contiguous() and v_pages.get_device() == dev,
@@ -73,7 +84,6 @@ def _cache(k_pages, v_pages, table, kv_lens, q_start):
     _need(page in _PAGES, "page must be a power of two from 8 to 1024, got %d", page)
     _need(dim in _DIMS, "head dim must be 64, 128 or 256, got %d", dim)
     _need(num_pages > 0 and heads > 0, "the cache has no pages or no heads")
-    tshape = table.shape
     _need(len(tshape) == 2 and tshape[1] > 0, "table must be [seqs, pages per sequence]")
     seqs = tshape[0]
     _int32(table, tshape, dev, "table")
@@ -84,31 +94,35 @@ def _cache(k_pages, v_pages, table, kv_lens, q_start):
 
 
 def _rows(t, heads, dim, dt, dev, what):
-    """-> the strides of the token and head axes"""
-    shape = t.shape
+    """-> tokens, heads and the strides of these two axes"""
+    shape, st = t.shape, t.stride()
+    if (len(shape) == 3 and shape[2] == dim and (heads is None or shape[1] == heads) and t.dtype is dt and t.get_device() == dev
+            and st[2] == 1 and not t.requires_grad):
+        return shape[0], shape[1], st[0], st[1]
     _need(len(shape) == 3 and shape[2] == dim and (heads is None or shape[1] == heads) and t.dtype is dt
           and t.get_device() == dev, "%s must be [tokens, %s, %d] %s on the cache's device", what,
           "heads" if heads is None else heads, dim, dt)
-    st = t.stride()
     _need(st[2] == 1 or t.numel() == 0, "%s must have contiguous rows of dim", what)
     _need(not t.requires_grad or not torch.is_grad_enabled(), _NO_GRAD, what)
-    return st[0], st[1]
+    return shape[0], shape[1], st[0], st[1]
 
 
 def paged_append(k_new, v_new, k_pages, v_pages, table, kv_lens, q_start=None):
     """writes the new tokens' keys and values [tokens, heads, dim] to their pages (positions kv_lens - n .. kv_lens - 1 of each
     sequence).  A token whose page the table does not name is dropped."""
     num_pages, heads, page, dim, seqs, ld, dt, dev = _cache(k_pages, v_pages, table, kv_lens, q_start)
-    ks, vs = _rows(k_new, heads, dim, dt, dev, "k_new"), _rows(v_new, heads, dim, dt, dev, "v_new")
-    tokens = k_new.shape[0]
-    _need(v_new.shape[0] == tokens, "k_new and v_new must have the same tokens")
-    _need(q_start is not None or seqs == 0 or tokens % seqs == 0, _EVEN, tokens, seqs)
-    _on_gpu(k_pages)
+    tokens, _, kt, kh = _rows(k_new, heads, dim, dt, dev, "k_new")
+    v_tokens, _, vt, vh = _rows(v_new, heads, dim, dt, dev, "v_new")
+    _need(v_tokens == tokens, "k_new and v_new must have the same tokens")
+    if q_start is None and seqs and tokens % seqs:
+        _need(False, _EVEN, tokens, seqs)
+    if dev < 0:
+        _on_gpu(k_pages)
     if tokens == 0 or seqs == 0:
         return
-    _launch(dev, "focr_paged_append", k_new.data_ptr(), v_new.data_ptr(), ks[0], ks[1], vs[0], vs[1], k_pages.data_ptr(),
-            v_pages.data_ptr(), table.data_ptr(), kv_lens.data_ptr(), None if q_start is None else q_start.data_ptr(), tokens,
-            seqs, heads, dim, page, ld, num_pages, _DTYPES[dt])
+    _launch(dev, "focr_paged_append", k_new.data_ptr(), v_new.data_ptr(), kt, kh, vt, vh, k_pages.data_ptr(), v_pages.data_ptr(),
+            table.data_ptr(), kv_lens.data_ptr(), None if q_start is None else q_start.data_ptr(), tokens, seqs, heads, dim, page,
+            ld, num_pages, _DTYPES[dt])
 
 
 def paged_attention(q, k_pages, v_pages, table, kv_lens, q_start=None, causal=True, scale=None, max_q=None, max_kv=None,
@@ -120,10 +134,10 @@ def paged_attention(q, k_pages, v_pages, table, kv_lens, q_start=None, causal=Tr
     given, positive.  max_q / max_kv: bounds on a sequence's new tokens and on kv_lens that the caller knows (they size the
     launch; the defaults are the most the tensors allow).  out: where to write (not q's memory)."""
     num_pages, kv_heads, page, dim, seqs, ld, dt, dev = _cache(k_pages, v_pages, table, kv_lens, q_start)
-    qs = _rows(q, None, dim, dt, dev, "q")
-    tokens, heads = q.shape[0], q.shape[1]
+    tokens, heads, qt, qh = _rows(q, None, dim, dt, dev, "q")
     _need(heads > 0 and heads % kv_heads == 0, "%d heads over a cache of %d", heads, kv_heads)
-    _need(q_start is not None or seqs == 0 or tokens % seqs == 0, _EVEN, tokens, seqs)
+    if q_start is None and seqs and tokens % seqs:
+        _need(False, _EVEN, tokens, seqs)
     scale = dim ** -0.5 if scale is None else float(scale)
     _need(0.0 < scale < math.inf, "scale must be positive and finite, got %r", scale)
     limit = min(ld * page, _LONGEST)
@@ -134,20 +148,21 @@ def paged_attention(q, k_pages, v_pages, table, kv_lens, q_start=None, causal=Tr
         max_q = tokens if max_q is None else min(int(max_q), tokens)
     _need(max_q >= 0 and max_kv >= 0, "max_q / max_kv out of range")
     if out is not None:
-        os = _rows(out, heads, dim, dt, dev, "out")
-        _need(out.shape[0] == tokens and os[0] != 0 and os[1] != 0, "out must have q's shape and rows of its own")
+        n, _, ot, oh = _rows(out, heads, dim, dt, dev, "out")
+        _need(n == tokens and ot != 0 and oh != 0, "out must have q's shape and rows of its own")
         _need(not _overlap(out, q), "out must not share q's memory")
-    _on_gpu(k_pages)
+    if dev < 0:
+        _on_gpu(k_pages)
     if out is None:
-        out, os = torch.empty((tokens, heads, dim), dtype=dt, device=q.device), (heads * dim, dim)
+        out, ot, oh = torch.empty((tokens, heads, dim), dtype=dt, device=q.device), heads * dim, dim
     if tokens == 0 or seqs == 0:
         return out
     code = _DTYPES[dt]
     n_ws = _lib.load().focr_paged_attention_ws_bytes(tokens, seqs, heads, kv_heads, dim, max_q, max_kv, code)
     _need(n_ws >= 0, "arguments out of range")
     ws = torch.empty(n_ws, dtype=torch.uint8, device=q.device) if n_ws else None
-    _launch(dev, "focr_paged_attention_fwd", q.data_ptr(), qs[0], qs[1], k_pages.data_ptr(), v_pages.data_ptr(),
-            table.data_ptr(), kv_lens.data_ptr(), None if q_start is None else q_start.data_ptr(), out.data_ptr(), os[0], os[1],
+    _launch(dev, "focr_paged_attention_fwd", q.data_ptr(), qt, qh, k_pages.data_ptr(), v_pages.data_ptr(),
+            table.data_ptr(), kv_lens.data_ptr(), None if q_start is None else q_start.data_ptr(), out.data_ptr(), ot, oh,
             None if ws is None else ws.data_ptr(), n_ws, tokens, seqs, heads, kv_heads, dim, page, ld, num_pages, max_q, max_kv,
             scale, 1 if causal else 0, code)
     return out
@@ -175,23 +190,26 @@ def beam_select(logits, scores, finished=None, eos=None, n=None):
     _need(len(shape) == 3 and dt in _DTYPES, "logits must be [batch, beams, vocab] in fp32, bf16 or fp16")
     batch, beams, vocab = shape
     n = beams if n is None else int(n)
-    _need(1 <= beams <= 64 and 1 <= n <= 64 and vocab >= 1 and n <= beams * vocab,
-          "beams and n must be 1 to 64 and n at most beams * vocab; got %d beams, n = %d, vocab %d", beams, n, vocab)
-    ls = logits.stride()
+    if not (1 <= beams <= 64 and 1 <= n <= 64 and vocab >= 1 and n <= beams * vocab):
+        _need(False, "beams and n must be 1 to 64 and n at most beams * vocab; got %d beams, n = %d, vocab %d", beams, n, vocab)
+    ls, rows = logits.stride(), (batch, beams)
     _need(ls[2] == 1 or vocab == 1 or logits.numel() == 0, "logits must have contiguous rows of vocab")
     _need(not logits.requires_grad or not torch.is_grad_enabled(), _NO_GRAD, "logits")
-    _need(scores.dtype is torch.float32 and scores.shape == (batch, beams) and scores.is_contiguous()
-          and scores.get_device() == dev, "scores must be a contiguous fp32 tensor [batch, beams] on the logits' device")
+    _need(scores.dtype is torch.float32 and scores.shape == rows and scores.is_contiguous() and scores.get_device() == dev,
+          "scores must be a contiguous fp32 tensor [batch, beams] on the logits' device")
     if finished is not None:
-        _need(finished.dtype is torch.bool and finished.shape == (batch, beams) and finished.is_contiguous()
-              and finished.get_device() == dev, "finished must be a contiguous bool tensor [batch, beams] on the logits' device")
+        _need(finished.dtype is torch.bool and finished.shape == rows and finished.is_contiguous() and finished.get_device() == dev,
+              "finished must be a contiguous bool tensor [batch, beams] on the logits' device")
         _need(eos is not None, "finished beams need an eos")
     _need(eos is None or 0 <= int(eos) < vocab, "eos must be inside the vocabulary")
     eos = -1 if eos is None else int(eos)
-    _on_gpu(logits)
+    if dev < 0:
+        _on_gpu(logits)
     device = logits.device
-    out_scores, out_parents = (torch.empty((batch, n), dtype=t, device=device) for t in (torch.float32, torch.int32))
-    out_tokens, out_finished = (torch.empty((batch, n), dtype=t, device=device) for t in (torch.int64, torch.bool))
+    out_scores = torch.empty_like(scores) if n == beams else torch.empty((batch, n), dtype=torch.float32, device=device)
+    out_parents = torch.empty_like(out_scores, dtype=torch.int32)
+    out_tokens = torch.empty_like(out_scores, dtype=torch.int64)
+    out_finished = torch.empty_like(out_scores, dtype=torch.bool)
     if batch:
         code = _DTYPES[dt]
         n_ws = _lib.load().focr_beam_select_ws_bytes(batch, beams, vocab, n, code)
@@ -227,18 +245,24 @@ def beam_reorder(parents, table, kv_lens, spare, pages, table_out=None, spare_ou
     _need(len(pages) > 0, "no page tensors")
     shape, dt = pages[0].shape, pages[0].dtype
     for p in pages:
-        _need(len(shape) == 4 and p.shape == shape and p.dtype is dt and dt in _DTYPES and p.is_contiguous()
-              and p.get_device() == dev, "pages must be contiguous [num_pages, heads, page, dim] tensors of one shape and type "
-              "(fp32, bf16 or fp16) on the parents' device")
+        if not (len(shape) == 4 and p.shape == shape and p.dtype is dt and dt in _DTYPES and p.is_contiguous()
+                and p.get_device() == dev):
+            _need(False, "pages must be contiguous [num_pages, heads, page, dim] tensors of one shape and type (fp32, bf16 or "
+                  "fp16) on the parents' device")
     num_pages, heads, page, dim = shape
     _need(page in _PAGES, "page must be a power of two from 8 to 1024, got %d", page)
     _need(num_pages > 0 and heads > 0 and dim > 0 and dim * pages[0].element_size() % 16 == 0,
           "rows of dim must be whole 16-byte units")
-    table_out = torch.empty_like(table) if table_out is None else table_out
-    spare_out = torch.empty_like(spare) if spare_out is None else spare_out
-    _int32(table_out, tshape, dev, "table_out")
-    _int32(spare_out, (slots,), dev, "spare_out")
-    _on_gpu(parents)
+    if table_out is None:
+        table_out = torch.empty_like(table)
+    else:
+        _int32(table_out, tshape, dev, "table_out")
+    if spare_out is None:
+        spare_out = torch.empty_like(spare)
+    else:
+        _int32(spare_out, (slots,), dev, "spare_out")
+    if dev < 0:
+        _on_gpu(parents)
     if slots:
         ptrs = (ctypes.c_void_p * len(pages))(*[p.data_ptr() for p in pages])
         _launch(dev, "focr_beam_reorder", parents.data_ptr(), table.data_ptr(), kv_lens.data_ptr(), spare.data_ptr(),
