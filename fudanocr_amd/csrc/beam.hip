@@ -517,8 +517,13 @@ extern "C" int focr_beam_reorder(const int* parents, const int* table, const int
   for (int i = 0; i < tensors; ++i) FOCR_CHECK_ARG(pages[i] && ((uintptr_t)pages[i] & 15) == 0, "pages must be 16-byte aligned");
   const int shift = __builtin_ctz(page);
   const long slots = (long)groups * beams;
-  const bool apart = (table_out + slots * table_ld <= table || table + slots * table_ld <= table_out) &&
-                     (spare_out + slots <= spare || spare + slots <= spare_out);
+  const long tb = slots * table_ld * 4, sb = slots * 4;
+  const bool t_apart = !focr_overlap(table_out, tb, table, tb), s_apart = !focr_overlap(spare_out, sb, spare, sb), apart = t_apart && s_apart;
+  FOCR_CHECK_ARG((t_apart || table_out == table) && (s_apart || spare_out == spare) && !focr_overlap(table_out, tb, spare_out, sb) &&
+                     !focr_overlap(table_out, tb, spare, sb) && !focr_overlap(spare_out, sb, table, tb) &&
+                     !focr_overlap(table_out, tb, parents, sb) && !focr_overlap(spare_out, sb, parents, sb) &&
+                     !focr_overlap(table_out, tb, kv_lens, sb) && !focr_overlap(spare_out, sb, kv_lens, sb),
+                 "table_out / spare_out share memory with another argument (they may be table / spare themselves)");
   for (int i = 0; i < tensors; i += BR_MAX_TENSORS) {
     BrPages b = {};
     const int m = tensors - i < BR_MAX_TENSORS ? tensors - i : BR_MAX_TENSORS;

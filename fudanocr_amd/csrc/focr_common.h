@@ -44,6 +44,11 @@ extern "C" int focr_get_tuning(int key);
     }                                                                    \
   } while (0)
 
+// do [a, a + na) and [b, b + nb) bytes share any
+static inline bool focr_overlap(const void* a, long na, const void* b, long nb) {
+  return na > 0 && nb > 0 && (const char*)a < (const char*)b + nb && (const char*)b < (const char*)a + na;
+}
+
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(2))) float f32x2;

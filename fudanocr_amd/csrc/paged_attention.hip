@@ -946,7 +946,12 @@ extern "C" int focr_paged_append(const void* k_new, const void* v_new, long ldtk
   PagedShape c;
   FOCR_CHECK_ARG(pg_shape(c, table, kv_lens, q_start, tokens, seqs, page, table_ld, num_pages, INT32_MAX),
                  "page must be a power of two from 8 to 1024");
-  const long es = pg_esize(dtype);
+  const long es = pg_esize(dtype), cache = num_pages * heads * page * dim * es;
+  const long kb = ((tokens - 1) * ldtk + (heads - 1) * ldhk + dim) * es, vb = ((tokens - 1) * ldtv + (heads - 1) * ldhv + dim) * es;
+  FOCR_CHECK_ARG(!focr_overlap(k_pages, cache, v_pages, cache), "k_pages and v_pages share memory");
+  FOCR_CHECK_ARG(!focr_overlap(k_new, kb, k_pages, cache) && !focr_overlap(k_new, kb, v_pages, cache) &&
+                     !focr_overlap(v_new, vb, k_pages, cache) && !focr_overlap(v_new, vb, v_pages, cache),
+                 "the new tokens share memory with the cache");
   const long strides = ldtk | ldhk | ldtv | ldhv;
   const bool wide = pg_aligned(k_new) && pg_aligned(v_new) && ((strides * es) & 15) == 0;
   auto kern = wide ? paged_append_kernel<16> : es == 4 ? paged_append_kernel<4> : paged_append_kernel<2>;
@@ -1093,9 +1098,13 @@ extern "C" int focr_paged_attention_fwd(const void* q, long ldt, long ldh, const
   PagedShape c;
   FOCR_CHECK_ARG(pg_shape(c, table, kv_lens, q_start, tokens, seqs, page, table_ld, num_pages, max_kv),
                  "page must be a power of two from 8 to 1024");
+  const long es = pg_esize(dtype), cache = num_pages * kv_heads * page * dim * es;
+  const long qb = ((tokens - 1) * ldt + (heads - 1) * ldh + dim) * es, ob = ((tokens - 1) * ldto + (heads - 1) * ldho + dim) * es;
+  FOCR_CHECK_ARG(!focr_overlap(o, ob, q, qb) && !focr_overlap(o, ob, k_pages, cache) && !focr_overlap(o, ob, v_pages, cache),
+                 "the output shares memory with q or the cache");
   int rc;
-  const bool wq = pg_aligned(q) && (((ldt | ldh) * pg_esize(dtype)) & 15) == 0;
-  const bool wo = pg_aligned(o) && (((ldto | ldho) * pg_esize(dtype)) & 15) == 0;
+  const bool wq = pg_aligned(q) && (((ldt | ldh) * es) & 15) == 0;
+  const bool wo = pg_aligned(o) && (((ldto | ldho) * es) & 15) == 0;
 #define PG_RUN(T, DD)                                                                                                       \
   rc = pg_run<T, DD>(PgArgs<T>{(const T*)q, ldt, ldh, (const T*)k_pages, (const T*)v_pages, c, (T*)o, ldto, ldho, (float*)ws, \
                                nullptr, max_q, heads, kv_heads, heads / kv_heads, 1, 0, 0, 0, causal ? 1 : 0, 0, wq, wo,             \

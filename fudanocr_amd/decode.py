@@ -74,7 +74,8 @@ def _cache(k_pages, v_pages, table, kv_lens, q_start):
             and table.is_contiguous() and table.get_device() == dev and kv_lens.dtype is torch.int32
             and kv_lens.shape == (tshape[0],) and kv_lens.is_contiguous() and kv_lens.get_device() == dev
             and (q_start is None or (q_start.dtype is torch.int32 and q_start.shape == (tshape[0] + 1,)
-                                     and q_start.is_contiguous() and q_start.get_device() == dev))):
+                                     and q_start.is_contiguous() and q_start.get_device() == dev))
+            and not k_pages.requires_grad and not v_pages.requires_grad):
         return *shape, *tshape, dt, dev
     _need(len(shape) == 4 and shape == v_pages.shape and dt is v_pages.dtype and dt in _DTYPES,
           "k_pages and v_pages must be two [num_pages, heads, page, dim] tensors of one type (fp32, bf16 or fp16)")
@@ -90,6 +91,7 @@ def _cache(k_pages, v_pages, table, kv_lens, q_start):
     _int32(kv_lens, (seqs,), dev, "kv_lens")
     if q_start is not None:
         _int32(q_start, (seqs + 1,), dev, "q_start")
+    _need(not (k_pages.requires_grad or v_pages.requires_grad) or not torch.is_grad_enabled(), _NO_GRAD, "the cache")
     return num_pages, heads, page, dim, seqs, tshape[1], dt, dev
 
 
@@ -109,7 +111,7 @@ def _rows(t, heads, dim, dt, dev, what):
 
 def paged_append(k_new, v_new, k_pages, v_pages, table, kv_lens, q_start=None):
     """writes the new tokens' keys and values [tokens, heads, dim] to their pages (positions kv_lens - n .. kv_lens - 1 of each
-    sequence).  A token whose page the table does not name is dropped."""
+    sequence).  A token whose page the table does not name is dropped.  k_pages, v_pages and the new tokens lie apart."""
     num_pages, heads, page, dim, seqs, ld, dt, dev = _cache(k_pages, v_pages, table, kv_lens, q_start)
     tokens, _, kt, kh = _rows(k_new, heads, dim, dt, dev, "k_new")
     v_tokens, _, vt, vh = _rows(v_new, heads, dim, dt, dev, "v_new")
@@ -132,7 +134,7 @@ def paged_attention(q, k_pages, v_pages, table, kv_lens, q_start=None, causal=Tr
     heads is a multiple of the cache's; head h reads the cache's head h // (heads / cache heads).  causal: a token at position p
     sees the positions 0 .. p, else all kv_lens of them; a token that sees nothing gets zeros.  scale: 1 / sqrt(dim) unless
     given, positive.  max_q / max_kv: bounds on a sequence's new tokens and on kv_lens that the caller knows (they size the
-    launch; the defaults are the most the tensors allow).  out: where to write (not q's memory)."""
+    launch; the defaults are the most the tensors allow).  out: where to write (apart from q and the cache)."""
     num_pages, kv_heads, page, dim, seqs, ld, dt, dev = _cache(k_pages, v_pages, table, kv_lens, q_start)
     tokens, heads, qt, qh = _rows(q, None, dim, dt, dev, "q")
     _need(heads > 0 and heads % kv_heads == 0, "%d heads over a cache of %d", heads, kv_heads)
@@ -149,7 +151,8 @@ def paged_attention(q, k_pages, v_pages, table, kv_lens, q_start=None, causal=Tr
     _need(max_q >= 0 and max_kv >= 0, "max_q / max_kv out of range")
     if out is not None:
         n, _, ot, oh = _rows(out, heads, dim, dt, dev, "out")
-        _need(n == tokens and ot != 0 and oh != 0, "out must have q's shape and rows of its own")
+        _need(n == tokens and ((tokens == 1 or ot >= (heads - 1) * oh + dim) and (heads == 1 or oh >= dim)
+                               or ot >= dim and oh >= (tokens - 1) * ot + dim), "out must have q's shape and rows of its own")
         _need(not _overlap(out, q), "out must not share q's memory")
     if dev < 0:
         _on_gpu(k_pages)
@@ -194,7 +197,7 @@ def beam_select(logits, scores, finished=None, eos=None, n=None):
         _need(False, "beams and n must be 1 to 64 and n at most beams * vocab; got %d beams, n = %d, vocab %d", beams, n, vocab)
     ls, rows = logits.stride(), (batch, beams)
     _need(ls[2] == 1 or vocab == 1 or logits.numel() == 0, "logits must have contiguous rows of vocab")
-    _need(not logits.requires_grad or not torch.is_grad_enabled(), _NO_GRAD, "logits")
+    _need(not (logits.requires_grad or scores.requires_grad) or not torch.is_grad_enabled(), _NO_GRAD, "logits or scores")
     _need(scores.dtype is torch.float32 and scores.shape == rows and scores.is_contiguous() and scores.get_device() == dev,
           "scores must be a contiguous fp32 tensor [batch, beams] on the logits' device")
     if finished is not None:
@@ -228,8 +231,8 @@ def beam_reorder(parents, table, kv_lens, spare, pages, table_out=None, spare_ou
     kv_lens (the first one's counts).  Full pages are shared by table entry; the partial last page is copied to the beam's page
     in `spare` (int32 [seqs]), and the one it had becomes its spare.  pages: the page tensors (k_pages and v_pages of every
     layer) that the table stands for.  Before the call, the pages in `spare` and each beam's entries from its partial page on
-    must be its own alone (`PagedCache` sees to that).  table_out / spare_out may be the inputs; a parent outside
-    the group counts as the beam itself."""
+    must be its own alone (`PagedCache` sees to that).  table_out / spare_out are the inputs or lie apart from them; a parent
+    outside the group counts as the beam itself."""
     pshape, dev = parents.shape, parents.get_device()
     _need(len(pshape) == 2, "parents must be [groups, beams]")
     groups, beams = pshape
@@ -249,6 +252,7 @@ def beam_reorder(parents, table, kv_lens, spare, pages, table_out=None, spare_ou
                 and p.get_device() == dev):
             _need(False, "pages must be contiguous [num_pages, heads, page, dim] tensors of one shape and type (fp32, bf16 or "
                   "fp16) on the parents' device")
+        _need(not p.requires_grad or not torch.is_grad_enabled(), _NO_GRAD, "a page tensor")
     num_pages, heads, page, dim = shape
     _need(page in _PAGES, "page must be a power of two from 8 to 1024, got %d", page)
     _need(num_pages > 0 and heads > 0 and dim > 0 and dim * pages[0].element_size() % 16 == 0,

@@ -76,9 +76,8 @@ class Transformer(nn.Module):
         """the `beams` most likely stroke strings of every image: (tokens int64 [B, beams, max_len], log-probabilities fp32 [B,
         beams]), best first, closed with '0' (fudanocr_amd/sld/beam.py).  image NCHW [B, 1 or 4, 32, 128]; eval mode."""
         from ..sld import beam
-        with torch.no_grad():
-            if image.shape[1] == 4:
-                image = K.bicubic_gray(image, image.shape[3])
-            feat = self.encoder(image)
-        return beam.search(self, feat, self.embedding_word_with_upperword, self.generator_word_with_upperword, beams, max_len,
+
+        def encode():
+            return self.encoder(K.bicubic_gray(image, image.shape[3]) if image.shape[1] == 4 else image)
+        return beam.search(self, encode, self.embedding_word_with_upperword, self.generator_word_with_upperword, beams, max_len,
                            alphabet.index("0"), alphabet.index("0"))

@@ -17,9 +17,10 @@ def _norm(ln, x, residual):
 
 
 @torch.no_grad()
-def search(model, feat, embedding, generator, beams, max_len, start, eos):
-    """feat NHWC [B, H, W, 1024] (the encoder's output) -> (tokens int64 [B, beams, max_len], scores fp32 [B, beams]), best first.
-    A hypothesis ends with its first `eos`; the positions behind it hold `eos` too.  Nothing in here waits for the device."""
+def search(model, encode, embedding, generator, beams, max_len, start, eos):
+    """encode() -> the encoder's output NHWC [B, H, W, 1024], called once the arguments are checked -> (tokens
+    int64 [B, beams, max_len], scores fp32 [B, beams]), best first.  A hypothesis ends with its first `eos`; the positions behind
+    it hold `eos` too.  Nothing in here waits for the device."""
     if model.training:
         raise RuntimeError("beam_search needs the model in eval mode")
     if not (1 <= beams <= 64 and max_len >= 1 and max_len <= model.pe.pe.shape[1]):
@@ -27,6 +28,7 @@ def search(model, feat, embedding, generator, beams, max_len, start, eos):
     vocab = generator.proj.weight.shape[0]
     if not (0 <= start < vocab and 0 <= eos < vocab):
         raise RuntimeError("beam_search: start and eos must be inside the %d classes" % vocab)
+    feat = encode()
     dec, dev = model.decoder, feat.device
     own, cross = dec.mask_multihead, dec.multihead
     batch, hh, ww, dm = feat.shape

@@ -256,7 +256,8 @@ class Transformer(nn.Module):
         call; eval mode."""
         from .. import beam
         alphabet = get_alphabet(self.mode)
-        with torch.no_grad():
-            feat = self.encoder(K.to_nhwc(image)) if conv_feature is None else K.to_nhwc(conv_feature)
-        return beam.search(self, feat, self.embedding_word, self.generator_word, beams, max_len, alphabet.index("<"),
+
+        def encode():
+            return self.encoder(K.to_nhwc(image)) if conv_feature is None else K.to_nhwc(conv_feature)
+        return beam.search(self, encode, self.embedding_word, self.generator_word, beams, max_len, alphabet.index("<"),
                            alphabet.index("$"))

@@ -481,7 +481,7 @@ int focr_weight_cross_entropy_masked_fwd(const float* logits, const long long* t
  * token and head axes (rows of dim contiguous).  Pages [num_pages][heads][page][dim], page a power of two 8..1024, dim 64 / 128 /
  * 256; table [seqs][table_ld], kv_lens [seqs] (new tokens included), q_start [seqs + 1] or NULL (tokens / seqs rows each): all
  * int32 in device memory and checked by the kernels -- a sequence whose numbers do not fit gets NaN, nothing outside the given
- * buffers is read or written. */
+ * buffers is read or written.  Outputs and pages share no memory with what is read. */
 #define FOCR_DT_F32 0
 #define FOCR_DT_BF16 1
 #define FOCR_DT_F16 2
@@ -502,7 +502,7 @@ int focr_beam_select(const void* logits, long ldb, long ldk, const float* scores
                      int* out_parents, long long* out_tokens, uint8_t* out_finished, void* ws, long ws_bytes, int batch,
                      int beams, int vocab, int n, int eos, int dtype, focr_stream_t stream);
 /* parents [groups][beams]; slots = groups * beams rows of table / kv_lens / spare; pages: HOST array of `tensors` device
- * pointers to page tensors of one shape; table_out / spare_out may be table / spare */
+ * pointers to page tensors of one shape; table_out / spare_out may be table / spare, else share nothing */
 int focr_beam_reorder(const int* parents, const int* table, const int* kv_lens, const int* spare, int* table_out,
                       int* spare_out, void* const* pages, int tensors, int groups, int beams, int heads, int dim, int page,
                       int table_ld, long num_pages, int dtype, focr_stream_t stream);

@@ -807,3 +807,83 @@ def test_recognizer_beam_search_refusals():
     _raises("max_len", model.beam_search, image, max_len=7001)
     assert model.beam_search(image, beams=2, max_len=1)[0].shape == (1, 2, 1)
     _raises("eval mode", model.train().beam_search, image)
+
+
+# ------------------------------------------------------------------------------- refusals of shared memory and of gradients
+def test_beam_search_refuses_before_the_encoder_runs():
+    """a model in training mode is refused before its encoder could move the batch norms' running statistics"""
+    from fudanocr_amd.loss.transformer import Transformer as Characters
+    from fudanocr_amd.loss.transformer_english_decomposition import Transformer as EnglishStrokes
+    from fudanocr_amd.sld.model.transformer import Transformer as Strokes
+
+    def never(*a, **kw):
+        raise AssertionError("the encoder ran")
+    for model, image in ((Strokes("stroke"), torch.zeros(1, 3, 32, 32)), (Characters(), torch.zeros(1, 1, 32, 128)),
+                         (EnglishStrokes(), torch.zeros(1, 1, 32, 128))):
+        model.encoder.forward = never
+        _raises("eval mode", model.train().beam_search, image)
+        _raises("1 to 64", model.eval().beam_search, image, beams=65)
+        _raises("max_len", model.beam_search, image, max_len=0)
+
+
+def test_whatever_wants_a_gradient_is_refused():
+    c, q = _cpu_cache(), torch.zeros(3, 4, 64)
+    for i in (0, 1):
+        g = list(c)
+        g[i] = c[i].clone().requires_grad_(True)
+        _raises("wants a gradient", D.paged_attention, q, *g)
+        _raises("wants a gradient", D.paged_append, q[:, :2], q[:, :2], *g)
+        with torch.no_grad():
+            _raises("on the GPU", D.paged_attention, q, *g)
+    x, s = torch.zeros(2, 3, 7), torch.zeros(2, 3, requires_grad=True)
+    _raises("wants a gradient", D.beam_select, x, s)
+    p, t, sp = torch.zeros(2, 3, dtype=torch.int32), torch.zeros(6, 2, dtype=torch.int32), torch.zeros(6, dtype=torch.int32)
+    _raises("wants a gradient", D.beam_reorder, p, t, sp, sp, [torch.zeros(8, 2, 16, 64, requires_grad=True)])
+    with torch.no_grad():
+        _raises("on the GPU", D.beam_select, x, s)
+
+
+def test_outputs_whose_rows_overlap_are_refused():
+    c, q = _cpu_cache(), torch.zeros(3, 4, 64)
+    buf = torch.zeros(4096)
+    for strides in ((64, 64, 1), (256, 32, 1), (255, 64, 1), (64, 128, 1), (0, 64, 1), (256, 0, 1)):
+        _raises("rows of its own", D.paged_attention, q, *c, out=buf.as_strided((3, 4, 64), strides))
+    for strides in ((256, 64, 1), (64, 192, 1), (300, 70, 1)):        # apart: refused for being on the CPU alone
+        _raises("on the GPU", D.paged_attention, q, *c, out=buf.as_strided((3, 4, 64), strides))
+    _raises("on the GPU", D.paged_attention, q[:1], c[0], c[1], c[2][:1], c[3][:1], out=buf.as_strided((1, 4, 64), (0, 64, 1)))
+
+
+def test_c_entries_refuse_shared_memory():
+    """a result that lies in what is read, as addresses that are never followed: 8 pages x 2 heads x 16 x 64 fp32 = 64 KB"""
+    from fudanocr_amd import _lib
+    lib = _lib.load()
+    size, k, v, far = 65536, 1 << 20, 1 << 21, 1 << 24
+
+    def attend(q, o):
+        rc = lib.focr_paged_attention_fwd(q, 256, 64, k, v, far, far, None, o, 256, 64, None, 0, 3, 3, 4, 2, 64, 16, 2, 8, 1, 32, 0.1,
+                                          1, 0, None)
+        return rc, lib.focr_last_error().decode()
+
+    def append(kn, vn, kp=k, vp=v):
+        rc = lib.focr_paged_append(kn, vn, 128, 64, 128, 64, kp, vp, far, far, None, 3, 3, 2, 64, 16, 2, 8, 0, None)
+        return rc, lib.focr_last_error().decode()
+    rows = 3 * 256 * 4
+    for o in (k, k - rows + 16, k + size - 16, v, v + 4096, far + 2 * size + rows - 16, far + 2 * size):
+        rc, msg = attend(far + 2 * size, o)
+        assert rc == -1 and "share" in msg, (o, rc, msg)
+    rows = 3 * 128 * 4
+    for a, b in ((k, far), (far, v), (far, k + size - 16), (v - rows + 16, far), (far, k)):
+        rc, msg = append(a, b)
+        assert rc == -1 and "share" in msg, (a, b, rc, msg)
+    rc, msg = append(far, far, k, k + size - 16)
+    assert rc == -1 and "share" in msg, (rc, msg)
+    import ctypes
+    pages = (ctypes.c_void_p * 1)(k)
+
+    def reorder(table, spare, table_out, spare_out):
+        rc = lib.focr_beam_reorder(far, table, far, spare, table_out, spare_out, pages, 1, 2, 3, 2, 64, 16, 4, 8, 0, None)
+        return rc, lib.focr_last_error().decode()
+    t, s = v, v + 4096                                                # 6 x 4 entries = 96 bytes, 6 spares = 24
+    for table_out, spare_out in ((t + 16, s), (t - 80, s), (t, s + 4), (t, s - 20), (t, t + 92), (s - 92, s), (far, t), (t, far)):
+        rc, msg = reorder(t, s, table_out, spare_out)
+        assert rc == -1 and "share" in msg, (table_out, spare_out, rc, msg)
