@@ -16,14 +16,15 @@
 //   * per lane the running maximum and the sum of exp(x - maximum) in 64 bits.  The exponential is 13 full-rate fp64 operations
 //     (a multiple of ln 2 taken off by a rounding addition, a polynomial of degree 7 on the rest: 6e-11), about what the
 //     loads of 16-bit logits cost in time; a hardware exp2 in fp32 would be off by 1e-7, as far apart as neighbours can be;
-//   * a buffer of the values that may be among its n best, as 64-bit keys: the value's bits in an order that compares as integers,
-//     then the complement of the index.  The n-th largest of the lanes' running maxima is a lower bound of the n-th best, so
-//     little more than n values pass; they are appended by ballot, all lanes at once, and put in order at the end (placing each
-//     in a sorted list as it came took 14 us of the scan's 41 at 64 x 8 x 50001).
+//   * nothing else: afterwards the n-th largest of the lanes' maxima is a lower bound of the n-th best, only the few lanes whose
+//     maximum reaches it hold candidates, and their values are read again, 16 bytes a lane, all at once.  Little more than n pass;
+//     they are appended to a buffer by ballot, as 64-bit keys (the value's bits in an order that compares as integers, then the
+//     complement of the index), and put in order at the end.  (A bound that grows with the chunks, candidates taken from
+//     the registers: 45 us at 64 x 8 x 50001 where this takes 36.)
 // Segments start at fixed indices and lanes take fixed indices of them whatever the row's alignment, so equal rows have
 // equal sums.  A second pass over K x segments lists of n joins them (in the same block where a batch entry is small).
-// Measured (64 entries x 8 beams x 50001, bf16, 51 MB): scan 35 us -- 13 for the loads alone, 10 more for the exponentials, 12 for
-// the candidates, one after the other although four waves share a SIMD -- and 10 us for the join.
+// Measured (64 entries x 8 beams x 50001, bf16, 51 MB): scan 29 us -- 12 for the loads alone, 12 more for the exponentials, 5 for
+// the candidates -- and 7 us for the join.
 #define BS_CHUNK 2048
 #define BS_MAX 64                     // beams, and candidates asked for
 #define BS_WAVES 16                   // of the one-launch form
@@ -105,19 +106,19 @@ __device__ __forceinline__ void bs_trim(const u64_t* buf, int cnt, int n, int la
 
 template <typename T, int L>          // L loads of 16 bytes a lane make a chunk
 __device__ __forceinline__ void bs_scan(const T* row, int v0, int v1, int n, int lane, u64_t* buf, u64_t* best, BsStat& stat) {
-  constexpr int E = 16 / sizeof(T), CHUNK = L * 64 * E, G = L * E < 8 ? L * E : 8;      // G: values compared together
-  float m = -INFINITY, thr = -INFINITY;
+  constexpr int E = 16 / sizeof(T), CHUNK = L * 64 * E;
+  float m = -INFINITY, thr = -INFINITY, x[L * E];
   double sum = 0.0;
   bool nan = false, ahead = false;
-  int cnt = 0;
   bs_u32x4 w[L];
+  // 16 bytes of a row from `at` on; behind the row's end the last 16 of it, of which a lane takes what is its own
+  auto from = [&](int at) { return at + E <= v1 ? at : v1 - E; };
   auto load = [&](int base) {
 #pragma unroll
-    for (int j = 0; j < L; ++j) w[j] = *(const bs_u32x4_any*)(row + base + (j * 64 + lane) * E);
+    for (int j = 0; j < L; ++j) w[j] = *(const bs_u32x4_any*)(row + from(base + (j * 64 + lane) * E));
   };
   for (int base = v0; base < v1; base += CHUNK) {
-    float x[L * E];
-    if (base + CHUNK <= v1) {
+    if (v1 >= E) {
       if (!ahead) load(base);
 #pragma unroll
       for (int i = 0; i < L * E; ++i) {
@@ -125,28 +126,29 @@ __device__ __forceinline__ void bs_scan(const T* row, int v0, int v1, int n, int
         else x[i] = (float)__builtin_bit_cast(T, (uint16_t)(w[i / E][i % E / 2] >> (16 * (i & 1))));
         nan |= x[i] != x[i];
       }
-    } else {
+      if (base + CHUNK > v1) {
+#pragma unroll
+        for (int i = 0; i < L * E; ++i) {
+          const int at = base + (i / E * 64 + lane) * E;
+          if (from(at) + i % E < at) x[i] = NAN;                  // another lane's: passes no comparison, adds nothing
+        }
+      }
+    } else {                                                      // a row of less than 16 bytes: in lane 0
 #pragma unroll
       for (int i = 0; i < L * E; ++i) {
-        const int v = base + ((i / E) * 64 + lane) * E + i % E;
-        x[i] = NAN;                                               // none: passes no comparison, adds nothing
-        if (v < v1) {
-          x[i] = (float)row[v];
-          nan |= x[i] != x[i];
+        x[i] = NAN;
+        if (i < E) {
+          const float y = (float)row[i < v1 ? i : v1 - 1];
+          nan |= y != y;
+          if (i < v1 && lane == 0) x[i] = y;
         }
       }
     }
-    ahead = base + 2 * CHUNK <= v1;
+    ahead = base + CHUNK < v1;
     if (ahead) load(base + CHUNK);                                // under this chunk's arithmetic
-    float gm[L * E / G], cm = -INFINITY;
+    float cm = -INFINITY;
 #pragma unroll
-    for (int g = 0; g < L * E / G; ++g) {
-      gm[g] = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < G; ++i) gm[g] = fmaxf(gm[g], x[g * G + i]);
-      cm = fmaxf(cm, gm[g]);
-    }
-    const bool better = __ballot(cm >= thr) != 0;
+    for (int i = 0; i < L * E; ++i) cm = fmaxf(cm, x[i]);
     if (cm > m) {
       sum *= bs_exp((double)m - (double)cm);                      // (-inf before the first values: the sum is 0)
       m = cm;
@@ -157,64 +159,100 @@ __device__ __forceinline__ void bs_scan(const T* row, int v0, int v1, int n, int
       sum += bs_exp((double)x[i] - ref);                          // (-inf: 1e-304, nothing beside the maximum's 1)
       if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);          // four chains at a time fill the pipe; more only take registers
     }
-    if (!better) continue;
+  }
 
-    if (v1 - v0 > 256) {                                          // the n-th largest of the lanes' maxima: values that are there
-      float t = -INFINITY;
-      if (n <= 16) {
-        float y = m;
-        for (int r = 0; r < n; ++r) {
-          t = bs_wave_max(y);
-          if (lane == __builtin_ctzll(__ballot(y == t) | 1ull << 63)) y = -INFINITY;
-        }
-      } else {
-        int rank = 0;
+  if (L > 1 || v1 - v0 > 256) {                                   // the n-th largest of the lanes' maxima: values that are there
+    if (n <= 16) {
+      float y = m;
+      for (int r = 0; r < n; ++r) {
+        thr = bs_wave_max(y);
+        if (lane == __builtin_ctzll(__ballot(y == thr) | 1ull << 63)) y = -INFINITY;
+      }
+    } else {
+      int rank = 0;
 #pragma unroll 8
-        for (int j = 0; j < 64; ++j) {
-          const float y = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m), j));
-          rank += y > m || (y == m && j < lane);
-        }
-        t = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m), __builtin_ctzll(__ballot(rank == n - 1) | 1ull << 63)));
+      for (int j = 0; j < 64; ++j) {
+        const float y = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m), j));
+        rank += y > m || (y == m && j < lane);
       }
-      thr = fmaxf(thr, t);
-    }
-    const int before = cnt;
-#pragma unroll
-    for (int g = 0; g < L * E / G; ++g) {
-      if (!__ballot(gm[g] >= thr)) continue;
-#pragma unroll
-      for (int i = g * G; i < g * G + G; ++i) {
-        const bool take = x[i] >= thr;
-        const u64_t pass = __ballot(take);
-        if (!pass) continue;
-        if (take && cnt + __popcll(pass) <= BS_BUF)
-          buf[cnt + __builtin_amdgcn_mbcnt_hi((uint32_t)(pass >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)pass, 0))] =
-              bs_key(x[i], base + ((i / E) * 64 + lane) * E + i % E);
-        cnt += __popcll(pass);
-      }
-    }
-    __builtin_amdgcn_wave_barrier();
-    if (cnt > BS_BUF / 2) {
-      // Rarely (many equal values, or ever better ones): the buffer goes back to its n best; if it ran over, this chunk's values
-      // are gone through again, 64 at a time, and placed one by one in the sorted list
-      const bool over = cnt > BS_BUF;
-      bs_trim(buf, over ? before : cnt, n, lane, best);
-      u64_t list = lane < n ? best[lane] : 0;
-      for (int v = base + lane; over && v - lane < v1 && v - lane < base + CHUNK; v += 64) {
-        const u64_t key = v < v1 ? bs_key((float)row[v], v) : 0;
-        u64_t pass = __ballot(key > bs_lane(list, n - 1));
-        while (pass) {
-          const int l = __builtin_ctzll(pass);
-          pass &= pass - 1;
-          bs_insert(list, bs_lane(key, l), lane);
-        }
-      }
-      if (lane < n) buf[lane] = list;
-      cnt = __popcll(__ballot(lane < n && list != 0));
-      if (cnt == n) thr = fmaxf(thr, bs_value(bs_lane(list, n - 1)));
-      __builtin_amdgcn_wave_barrier();
+      thr = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m), __builtin_ctzll(__ballot(rank == n - 1) | 1ull << 63)));
     }
   }
+  // Candidates to the buffer, a value a lane at a time.  Where they could run over (many equal values), the buffer goes back to
+  // its n best first and takes what is above the last of them
+  int cnt = 0;
+  u64_t least = 0;
+  auto put = [&](bool in, u64_t key) {
+    const u64_t pass = __ballot(in);
+    if (in) buf[cnt + __builtin_amdgcn_mbcnt_hi((uint32_t)(pass >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)pass, 0))] = key;
+    cnt += __popcll(pass);
+  };
+  auto take = [&](float (&y)[E], int (&v)[E]) {
+    int more = 0;
+#pragma unroll
+    for (int j = 0; j < E; ++j) more += __popcll(__ballot(y[j] >= thr));
+    if (cnt + more <= BS_BUF) {
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (__ballot(y[j] >= thr)) put(y[j] >= thr, bs_key(y[j], v[j]));
+      return;
+    }
+#pragma unroll 1
+    for (int g = 0; g < E; ++g) {
+      if (cnt > BS_BUF - 64) {
+        __builtin_amdgcn_wave_barrier();
+        bs_trim(buf, cnt, n, lane, best);
+        const u64_t list = lane < n ? best[lane] : 0;
+        if (lane < n) buf[lane] = list;
+        cnt = n;
+        least = bs_lane(list, n - 1);
+        thr = bs_value(least);
+      }
+      put(y[0] >= thr && bs_key(y[0], v[0]) > least, bs_key(y[0], v[0]));
+#pragma unroll
+      for (int j = 1; j < E; ++j) y[j - 1] = y[j], v[j - 1] = v[j];
+    }
+  };
+  if (L == 1 || v1 < E) {                                         // a single chunk: the values are still there
+    float y[E];
+    int v[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) y[i] = x[i], v[i] = v1 >= E ? from(v0 + lane * E) + i : i;
+    take(y, v);
+  } else {
+    // only the lanes whose maximum reaches the threshold hold any.  Their values are read again by the whole wave, 16 bytes a lane
+    const bool has = m >= thr && lane * E < v1 - v0;
+    const u64_t some = __ballot(has);
+    const int rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(some >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)some, 0));
+    const int lanes = __popcll(some), pieces = (v1 - v0 + 64 * E - 1) / (64 * E), items = lanes * pieces;
+    const int who = __builtin_amdgcn_ds_permute(4 * (has ? rank : lanes + lane - rank), lane);      // those lanes first
+    for (int i0 = 0; i0 < items; i0 += 4 * 64) {
+      bs_u32x4 z[4];
+      int at[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {                               // four loads on their way together
+        const int i = i0 + j * 64 + lane, c = i / pieces, l = __builtin_amdgcn_ds_bpermute(4 * c, who);
+        at[j] = i < items ? v0 + ((i - c * pieces) * 64 + l) * E : v1;
+        z[j] = *(const bs_u32x4_any*)(row + from(at[j]));
+      }
+#pragma unroll 1
+      for (int j = 0; j < 4 && i0 + j * 64 < items; ++j) {
+        float y[E];
+        int v[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          if constexpr (sizeof(T) == 4) y[i] = __uint_as_float(z[0][i]);
+          else y[i] = (float)__builtin_bit_cast(T, (uint16_t)(z[0][i / 2] >> (16 * (i & 1))));
+          v[i] = from(at[0]) + i;
+          if (v[i] < at[0]) y[i] = NAN;
+        }
+        take(y, v);
+#pragma unroll
+        for (int k = 1; k < 4; ++k) z[k - 1] = z[k], at[k - 1] = at[k];
+      }
+    }
+  }
+  __builtin_amdgcn_wave_barrier();
   bs_trim(buf, cnt, n, lane, best);
   const float mx = bs_wave_max(m);
   sum = m == -INFINITY ? 0.0 : sum * bs_exp((double)m - (double)mx);
@@ -240,13 +278,26 @@ struct BsArgs {
 
 __device__ __forceinline__ bool bs_before(double ca, int ia, double cb, int ib) { return ca > cb || (ca == cb && ia < ib); }
 
-// Joins the lists of a batch entry (waves: of the block; lists / stats of this entry).  rc / rv [beams][n]: the rows' candidates
+struct BsBeam {
+  float score;
+  bool done;
+};
+__device__ __forceinline__ BsBeam bs_beam(const BsArgs& a, int b, int k) {
+  const int i = b * a.beams + (k < a.beams ? k : 0);
+  return {a.scores[i], a.fin && a.fin[i]};
+}
+
+// Joins the lists of a batch entry (waves: of the block; lists / stats of this entry; own: bs_beam of the wave's first beam).
+// rc / rv / rp [beams][n]: the rows' candidates and their places
 __device__ __forceinline__ void bs_join(const BsArgs& a, int b, const u64_t* lists, const BsStat* stats, double* rc, int* rv,
-                                        int waves) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = a.n;
+                                        int* rp, int waves, BsBeam own) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = a.n;
   const int have = n < a.vocab ? n : a.vocab;                     // candidates of a row
   for (int k = wave; k < a.beams; k += waves) {
+    const BsBeam beam = k == wave ? own : bs_beam(a, b, k);
     u64_t list = lane < n ? lists[(long)k * a.parts * n + lane] : 0;
+    BsStat first = {0.0, -INFINITY};                              // all loads before the work on any
+    if (lane < a.parts) first = stats[k * a.parts + lane];
     for (int p0 = 1; p0 < a.parts; p0 += 8) {                     // eight loads at a time, then their turn
       u64_t other[8];
 #pragma unroll
@@ -260,22 +311,22 @@ __device__ __forceinline__ void bs_join(const BsArgs& a, int b, const u64_t* lis
           bs_insert(list, key, lane);
         }
     }
-    float m = -INFINITY;
-    double sum = 0.0;
-    bool nan = false;
-    for (int p = lane; p < a.parts; p += 64) {
+    float m = first.max;
+    bool nan = m != m;
+    for (int p = 64 + lane; p < a.parts; p += 64) {
       const float x = stats[k * a.parts + p].max;
       nan |= x != x;
       m = fmaxf(m, x);
     }
-    m = wave_max(m);
-    for (int p = lane; p < a.parts; p += 64) {
+    m = bs_wave_max(m);
+    double sum = first.max > -INFINITY ? first.sum * bs_exp((double)first.max - (double)m) : 0.0;
+    for (int p = 64 + lane; p < a.parts; p += 64) {
       const BsStat st = stats[k * a.parts + p];
       if (st.max > -INFINITY) sum += st.sum * bs_exp((double)st.max - (double)m);
     }
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    const float s = a.scores[b * a.beams + k];
-    const bool done = a.fin && a.fin[b * a.beams + k];
+    const float s = beam.score;
+    const bool done = beam.done;
     const bool live = isfinite(s) && (done || (!__ballot(nan) && isfinite(m)));
     double c = -INFINITY;
     int v = lane;
@@ -296,32 +347,33 @@ __device__ __forceinline__ void bs_join(const BsArgs& a, int b, const u64_t* lis
     if (lane < have) {
       rc[k * n + at] = c;
       rv[k * n + at] = v;
+      rp[k * n + at] = done ? at | 1 << 30 : at;
     }
   }
   __syncthreads();
   // a candidate's place: its place in its own row plus, by bisection, how many of every other row come before it
-  for (int x = tid; x < a.beams * have; x += waves * 64) {
-    const int k = x / have, i = x - k * have;
+  const int all = a.beams * have;
+  for (int x = tid; x < all * a.beams; x += waves * 64) {
+    const int r = x / all, y = x - r * all, k = y / have, i = y - k * have;
+    if (r == k) continue;
     const double c = rc[k * n + i];
-    const int v = rv[k * n + i];
-    int at = i;
-    for (int r = 0; r < a.beams && at < n; ++r) {
-      if (r == k) continue;
-      int lo = 0, hi = have;
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        const double cm = rc[r * n + mid];
-        if (cm > c || (cm == c && r < k)) lo = mid + 1;
-        else hi = mid;
-      }
-      at += lo;
+    int lo = 0, hi = have;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      const double cm = rc[r * n + mid];
+      if (cm > c || (cm == c && r < k)) lo = mid + 1;
+      else hi = mid;
     }
-    if (at < n) {
-      a.out_scores[b * n + at] = (float)c;
-      a.out_parents[b * n + at] = k;
-      a.out_tokens[b * n + at] = v;
-      a.out_fin[b * n + at] = (a.fin && a.fin[b * a.beams + k]) || v == a.eos;
-    }
+    atomicAdd(&rp[k * n + i], lo);                                // whole numbers: the same in any order
+  }
+  __syncthreads();
+  for (int x = tid; x < all; x += waves * 64) {
+    const int k = x / have, i = k * n + x - k * have, at = rp[i] & (1 << 30) - 1, v = rv[i];
+    if (at >= n) continue;
+    a.out_scores[b * n + at] = (float)rc[i];
+    a.out_parents[b * n + at] = k;
+    a.out_tokens[b * n + at] = v;
+    a.out_fin[b * n + at] = rp[i] >> 30 || v == a.eos;
   }
 }
 
@@ -331,21 +383,23 @@ __global__ __launch_bounds__(64 * BS_WAVES) void beam_select_kernel(BsArgs a) {
   __shared__ u64_t buf[BS_WAVES * BS_BUF], lists[BS_WAVES * BS_MAX];
   __shared__ BsStat stats[BS_WAVES];
   __shared__ double rc[BS_WAVES * BS_MAX];
-  __shared__ int rv[BS_WAVES * BS_MAX];
-  const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, k = wave / a.parts, p = wave - k * a.parts;
+  __shared__ int rv[BS_WAVES * BS_MAX], rp[BS_WAVES * BS_MAX];
+  const int b = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int k = wave / a.parts, p = wave - k * a.parts;
+  const BsBeam own = bs_beam(a, b, wave);
   BsStat st;
   const int v0 = p * a.seg, v1 = v0 + a.seg < a.vocab ? v0 + a.seg : a.vocab;
   bs_scan<T, L>((const T*)a.logits + b * a.ldb + k * a.ldk, v0, v1, a.n, lane, buf + wave * BS_BUF, lists + wave * a.n, st);
   if (lane == 0) stats[wave] = st;
   __syncthreads();
-  bs_join(a, b, lists, stats, rc, rv, a.beams * a.parts);
+  bs_join(a, b, lists, stats, rc, rv, rp, a.beams * a.parts, own);
 }
 
 // the two-launch form
 template <typename T>
 __global__ __launch_bounds__(256, 4) void beam_scan_kernel(BsArgs a, int waves) {
   __shared__ u64_t buf[4 * BS_BUF], best[4 * BS_MAX];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = blockIdx.x * 4 + wave;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = blockIdx.x * 4 + wave;
   if (w >= waves) return;
   const int p = w % a.parts, row = w / a.parts, b = row / a.beams, k = row - b * a.beams;
   BsStat st;
@@ -356,14 +410,16 @@ __global__ __launch_bounds__(256, 4) void beam_scan_kernel(BsArgs a, int waves) 
   if (lane == 0) a.stats[w] = st;
 }
 __global__ __launch_bounds__(64 * BS_WAVES) void beam_join_kernel(BsArgs a, int waves) {
-  extern __shared__ double bs_rc[];                               // [beams][n], then the indices
+  extern __shared__ double bs_rc[];                               // [beams][n], then the indices, then the places
   const long rows = (long)blockIdx.x * a.beams * a.parts;
-  bs_join(a, blockIdx.x, a.lists + rows * a.n, a.stats + rows, bs_rc, (int*)(bs_rc + a.beams * a.n), waves);
+  int* rv = (int*)(bs_rc + a.beams * a.n);
+  bs_join(a, blockIdx.x, a.lists + rows * a.n, a.stats + rows, bs_rc, rv, rv + a.beams * a.n, waves,
+          bs_beam(a, blockIdx.x, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)));
 }
 
 // One launch with a block per batch entry while an entry has at most 16 K logits; else the rows are cut into segments of whole
-// chunks, about 4096 waves in all (64 x 8 x 50001 bf16: 2048 waves 51.6 us, 4096 49.6, 8192 51.2), and joined by a second
-// launch (64 x 5 x 6625 fp32: 18.7 us, in one launch 21.5).
+// chunks, about 2048 waves in all (64 x 8 x 50001 bf16: 36 us, 3072 or 4096 waves 38, 39), and joined by a second
+// launch (64 x 5 x 6625 fp32: 18.7 us, in one launch 21.5, both with a slower join).
 struct BsPlan {
   bool one;
   int parts, seg;
@@ -372,7 +428,7 @@ static BsPlan bs_plan(int batch, int beams, int vocab) {
   const int chunks = (vocab + BS_CHUNK - 1) / BS_CHUNK;
   BsPlan p;
   p.one = beams <= BS_WAVES && (long)beams * vocab <= 16384;
-  const long want = p.one ? BS_WAVES / beams : 4096 / ((long)batch * beams);
+  const long want = p.one ? BS_WAVES / beams : 2048 / ((long)batch * beams);
   const int per = want < 1 ? chunks : (int)((chunks + want - 1) / want);
   p.seg = per * BS_CHUNK;
   p.parts = (chunks + per - 1) / per;
@@ -413,7 +469,7 @@ extern "C" int focr_beam_select(const void* logits, long ldb, long ldk, const fl
     hipLaunchKernelGGL(kern, dim3(cdiv(rows, 4)), dim3(256), 0, st, a, (int)rows);
     FOCR_LAUNCH_CHECK();
     const int waves = beams < BS_WAVES ? beams : BS_WAVES;
-    hipLaunchKernelGGL(beam_join_kernel, dim3(batch), dim3(64 * waves), beams * n * 12, st, a, waves);
+    hipLaunchKernelGGL(beam_join_kernel, dim3(batch), dim3(64 * waves), beams * n * 16, st, a, waves);
   }
   FOCR_LAUNCH_CHECK();
   return FOCR_OK;
