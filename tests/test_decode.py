@@ -599,6 +599,47 @@ def test_selection_ties_masks_and_nonfinite(vocab):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("beams", [2, 20])
+def test_selection_at_the_ends_of_rows(dtype, beams):
+    """rows shorter than a 16-byte word, rows that end inside one, and rows that start at any element of one"""
+    for vocab in (1, 2, 3, 4, 5, 7, 8, 9, 15, 17, 255, 257, 511, 513, 2045, 2051, 8189, 8195, 14337):
+        g = torch.Generator().manual_seed(vocab)
+        n = min(beams * vocab, 11)
+        x = torch.randn(2, beams, vocab, generator=g).to(dtype)
+        x[:, :, vocab // 2:] += 2                                     # the best ones near the ends
+        s = -torch.rand(2, beams, generator=g)
+        check_select(x, s, n=n)
+        wide = torch.full((2, beams, vocab + 6), float("nan"), dtype=dtype)      # neighbours of a row that must not count
+        wide[:, :, 3:3 + vocab] = x
+        val, par, tok, fin = select_reference(x, s, None, -1, n)
+        got = D.beam_select(wide.cuda()[:, :, 3:3 + vocab], s.cuda(), n=n)
+        assert torch.equal(got[1].cpu(), par) and torch.equal(got[2].cpu(), tok), vocab
+        assert torch.isfinite(got[0]).all()
+
+
+@gpu
+@pytest.mark.parametrize("n", [1, 16, 17, 64])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_selection_of_many_equal_candidates(dtype, n):
+    """more values of one size than a wave's buffer holds: among the best ones, as the mask's value, everywhere, in either order"""
+    g = torch.Generator().manual_seed(n)
+    s = torch.tensor([[0.0, -0.5, -1.0]])
+    for vocab in (600, 20000, 70001):
+        x = torch.randn(1, 3, vocab, generator=g).clamp_max(0.5).to(dtype)
+        check_select(x, s, n=n)                                       # a third of them the maximum
+        for live in (1, 5, 40):                                       # a vocabulary masked to a few tokens
+            y = torch.full_like(x, float("-inf"))
+            y[:, :, torch.randperm(vocab, generator=g)[:live]] = 1.5
+            check_select(y, s, n=n)
+            check_select(torch.where(y == 1.5, x, torch.full_like(x, torch.finfo(dtype).min)), s, n=n)
+        check_select(torch.randint(0, 2, (1, 3, vocab), generator=g).to(dtype), s, n=n)
+        steps = (torch.arange(vocab) // 37).float().expand(1, 3, vocab) / 1024      # rising and falling in long steps
+        check_select(steps.to(dtype).contiguous(), s, n=n)
+        check_select(steps.flip(2).to(dtype).contiguous(), s, n=n)
+
+
+@gpu
 def test_selection_separates_neighbours_in_64_bits():
     """two beams whose candidates differ by less than fp32 resolves at that magnitude"""
     x = torch.randn(1, 2, 500, generator=torch.Generator().manual_seed(3))
