@@ -20,7 +20,8 @@
 //     maximum reaches it hold candidates, and their values are read again, 16 bytes a lane, all at once.  Little more than n pass;
 //     they are appended to a buffer by ballot, as 64-bit keys (the value's bits in an order that compares as integers, then the
 //     complement of the index), and put in order at the end.  (A bound that grows with the chunks, candidates taken from
-//     the registers: 45 us at 64 x 8 x 50001 where this takes 36.)
+//     the registers: 45 us at 64 x 8 x 50001 where this takes 36.)  Rows of nearly one value -- a vocabulary masked to a few
+//     tokens -- have all lanes read again, in order: 64 us at that size.
 // Segments start at fixed indices and lanes take fixed indices of them whatever the row's alignment, so equal rows have
 // equal sums.  A second pass over K x segments lists of n joins them (in the same block where a batch entry is small).
 // Measured (64 entries x 8 beams x 50001, bf16, 51 MB): scan 29 us -- 12 for the loads alone, 12 more for the exponentials, 5 for
@@ -91,16 +92,27 @@ __device__ __forceinline__ void bs_insert(u64_t& list, u64_t key, int lane) {
 // the ones above it
 __device__ __forceinline__ void bs_trim(const u64_t* buf, int cnt, int n, int lane, u64_t* out) {
   if (lane >= cnt && lane < n) out[lane] = 0;
-  for (int i = 0; i < cnt; i += 64) {
-    const u64_t mine = i + lane < cnt ? buf[i + lane] : 0;
-    int at = 0;
-    for (int j = 0; j < cnt; j += 64) {
-      const u64_t other = j + lane < cnt ? buf[j + lane] : 0;
-      const int m = cnt - j < 64 ? cnt - j : 64;
-      for (int e = 0; e < m; ++e) at += bs_lane(other, e) > mine;
+  constexpr int R = BS_BUF / 64;
+  u64_t mine[R];
+  int at[R] = {};
+#pragma unroll
+  for (int i = 0; i < R; ++i) mine[i] = i * 64 + lane < cnt ? buf[i * 64 + lane] : 0;
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    const int m = cnt - j * 64 < 64 ? cnt - j * 64 : 64;
+    if (cnt <= 64) {
+      for (int e = 0; e < m; ++e) at[0] += bs_lane(mine[j], e) > mine[0];
+    } else {
+      for (int e = 0; e < m; ++e) {
+        const u64_t key = bs_lane(mine[j], e);
+#pragma unroll
+        for (int i = 0; i < R; ++i) at[i] += key > mine[i];
+      }
     }
-    if (i + lane < cnt && at < n) out[at] = mine;
   }
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    if (i * 64 + lane < cnt && at[i] < n) out[at[i]] = mine[i];
   __builtin_amdgcn_wave_barrier();
 }
 
@@ -180,35 +192,41 @@ __device__ __forceinline__ void bs_scan(const T* row, int v0, int v1, int n, int
   }
   // Candidates to the buffer, a value a lane at a time.  Where they could run over (many equal values), the buffer goes back to
   // its n best first and takes what is above the last of them
-  int cnt = 0;
-  u64_t least = 0;
+  int cnt = 0, last = INT32_MAX;
   auto put = [&](bool in, u64_t key) {
     const u64_t pass = __ballot(in);
     if (in) buf[cnt + __builtin_amdgcn_mbcnt_hi((uint32_t)(pass >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)pass, 0))] = key;
     cnt += __popcll(pass);
   };
   auto take = [&](float (&y)[E], int (&v)[E]) {
-    int more = 0;
+    if (last == INT32_MAX) {                                      // the buffer was not cut yet: the bound alone counts
+      int more = 0;
 #pragma unroll
-    for (int j = 0; j < E; ++j) more += __popcll(__ballot(y[j] >= thr));
-    if (cnt + more <= BS_BUF) {
+      for (int j = 0; j < E; ++j) more += __popcll(__ballot(y[j] >= thr));
+      if (cnt + more <= BS_BUF) {
 #pragma unroll
-      for (int j = 0; j < E; ++j)
-        if (__ballot(y[j] >= thr)) put(y[j] >= thr, bs_key(y[j], v[j]));
-      return;
+        for (int j = 0; j < E; ++j)
+          if (__ballot(y[j] >= thr)) put(y[j] >= thr, bs_key(y[j], v[j]));
+        return;
+      }
     }
+    const auto fits = [&](float y, int v) { return y > thr || (y == thr && v < last); };
+    bool any = false;
+#pragma unroll
+    for (int j = 0; j < E; ++j) any |= fits(y[j], v[j]);
+    if (!__ballot(any)) return;
 #pragma unroll 1
     for (int g = 0; g < E; ++g) {
-      if (cnt > BS_BUF - 64) {
+      if (cnt > n + 64) {
         __builtin_amdgcn_wave_barrier();
         bs_trim(buf, cnt, n, lane, best);
         const u64_t list = lane < n ? best[lane] : 0;
         if (lane < n) buf[lane] = list;
         cnt = n;
-        least = bs_lane(list, n - 1);
-        thr = bs_value(least);
+        thr = bs_value(bs_lane(list, n - 1));
+        last = bs_index(bs_lane(list, n - 1));
       }
-      put(y[0] >= thr && bs_key(y[0], v[0]) > least, bs_key(y[0], v[0]));
+      put(fits(y[0], v[0]), bs_key(y[0], v[0]));
 #pragma unroll
       for (int j = 1; j < E; ++j) y[j - 1] = y[j], v[j - 1] = v[j];
     }
@@ -231,8 +249,8 @@ __device__ __forceinline__ void bs_scan(const T* row, int v0, int v1, int n, int
       int at[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {                               // four loads on their way together
-        const int i = i0 + j * 64 + lane, c = i / pieces, l = __builtin_amdgcn_ds_bpermute(4 * c, who);
-        at[j] = i < items ? v0 + ((i - c * pieces) * 64 + l) * E : v1;
+        const int i = i0 + j * 64 + lane, q = i / lanes, l = __builtin_amdgcn_ds_bpermute(4 * (i - q * lanes), who);
+        at[j] = i < items ? v0 + (q * 64 + l) * E : v1;
         z[j] = *(const bs_u32x4_any*)(row + from(at[j]));
       }
 #pragma unroll 1
