@@ -39,7 +39,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const char* __restric
                                                            long ldhk, long ldtv, long ldhv, char* __restrict__ kp,
                                                            char* __restrict__ vp, PagedShape c, int heads, int row_bytes) {
   const int lane = threadIdx.x & 63;
-  const long t = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const long t = (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (t >= c.tokens) return;
   const int s = pg_seq_of_row(c, t, lane);
   const PagedSeq q = paged_seq(c, s);
@@ -872,7 +872,7 @@ template <typename T, int D, int WPR>
 __global__ __launch_bounds__(256) void paged_join_kernel(PgArgs<T> a) {
   constexpr int E = D / 64;
   __shared__ float wmax[4], wsum[4], acc[3][D];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = wave % WPR;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % WPR;
   const long rows = a.c.tokens * a.heads;
   const int row = blockIdx.x * (4 / WPR) + wave / WPR;
   if (row >= rows) return;                             // (with 4 waves a row there is no such row)
