@@ -436,7 +436,7 @@ __global__ __launch_bounds__(64 * BS_WAVES) void beam_join_kernel(BsArgs a, int 
 }
 
 // One launch with a block per batch entry while an entry has at most 16 K logits; else the rows are cut into segments of whole
-// chunks, about 2048 waves in all (64 x 8 x 50001 bf16: 36 us, 3072 or 4096 waves 38, 39), and joined by a second
+// chunks, about 2048 waves in all (64 x 8 x 50001 bf16: 36 us, twice as many 39), and joined by a second
 // launch (64 x 5 x 6625 fp32: 18.7 us, in one launch 21.5, both with a slower join).
 struct BsPlan {
   bool one;
