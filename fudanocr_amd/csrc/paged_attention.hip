@@ -163,10 +163,25 @@ template <typename T> __device__ __forceinline__ float pg_weight(float s, float 
   else return __builtin_amdgcn_exp2f(fmaf(s, c2, (PgMma<T>::EXP == 0x7c00u ? 14.f : 0.f) - ref));
 }
 
-// a part's sum of weights relative to the common maximum; a part without keys has sum 0 at maximum -inf, one whose scores are
-// all NaN has a NaN sum there, which must not get lost
-__device__ __forceinline__ float pg_share(float sum, float log2_ratio) {
-  return sum == 0.f ? 0.f : sum != sum ? sum : sum * __builtin_amdgcn_exp2f(log2_ratio);
+// What the weights of a row are relative to, as its sums are kept and joined: the maximum itself in fp32, `ref` (the rounded
+// product, which every weight was taken against) in the 16-bit types.  Two of them are compared by their difference, so that sums
+// whose maximum stands are multiplied by 1 exactly: c2 m - ref in one multiply-add is the rounding error of c2 m there, once for
+// every other row of the wave that finds a new maximum, always with the same sign
+template <typename T> __device__ __forceinline__ float pg_top(float mx, float c2) { return sizeof(T) == 4 ? mx : mx * c2; }
+template <typename T> __device__ __forceinline__ float pg_ratio(float top, float to, float c2) {       // `to` above -inf
+  return __builtin_amdgcn_exp2f(sizeof(T) == 4 ? (top - to) * c2 : top - to);
+}
+// a running sum's factor when its maximum goes from m to mx; ref = c2 mx rounded, either 0 while there is no maximum
+template <typename T> __device__ __forceinline__ float pg_rescale(float m, float mx, float c2, float ref) {
+#pragma clang fp contract(off)
+  if constexpr (sizeof(T) == 4) return __builtin_amdgcn_exp2f((m - (mx == -INFINITY ? 0.f : mx)) * c2);
+  else return __builtin_amdgcn_exp2f(m * c2 - ref);
+}
+
+// a part's sum of weights at maximum `top` relative to the common one; a part without keys has sum 0 at maximum -inf, one whose
+// scores are all NaN has a NaN sum there, which must not get lost
+template <typename T> __device__ __forceinline__ float pg_share(float sum, float top, float to, float c2) {
+  return sum == 0.f ? 0.f : sum != sum ? sum : sum * pg_ratio<T>(top, to, c2);
 }
 
 template <typename T>
@@ -178,7 +193,7 @@ struct PgArgs {
   T* o;
   long ldto, ldho;
   float* part;   // [split][token][head][D], weights relative to the split's own maximum
-  float2* ml;    // [split][token][head]: that maximum (in log2 units) and the sum of the weights
+  float2* ml;    // [split][token][head]: that maximum (pg_top) and the sum of the weights
   int max_q, heads, kv_heads, group, nsplit, chunk, tile_chunk, tiles, causal, thin_rows, wide_q, wide_o;
   float c2;      // scale * log2(e)
 };
@@ -410,7 +425,7 @@ __global__ __launch_bounds__(256, (pg_thin_waves<T, D, NT>())) void paged_thin_k
       mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
       const float ref = mx == -INFINITY ? 0.f : mx * a.c2;
       if (__any(mx > m[t])) {
-        const float al = __builtin_amdgcn_exp2f(m[t] * a.c2 - ref);
+        const float al = pg_rescale<T>(m[t], mx, a.c2, ref);
         l[t] *= al;
 #pragma unroll
         for (int u = 0; u < VU; ++u)
@@ -496,14 +511,14 @@ __global__ __launch_bounds__(256, (pg_thin_waves<T, D, NT>())) void paged_thin_k
   for (int t = 0; t < NT; ++t) {
     l[t] += __shfl_xor(l[t], 16, 64);
     l[t] += __shfl_xor(l[t], 32, 64);
-    if (g == 0) wml[wave][t * 16 + l16] = float2{m[t], l[t]};
+    if (g == 0) wml[wave][t * 16 + l16] = float2{pg_top<T>(m[t], a.c2), l[t]};
   }
   __syncthreads();
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     float mx = wml[0][t * 16 + l16].x;
     for (int w = 1; w < nw; ++w) mx = fmaxf(mx, wml[w][t * 16 + l16].x);
-    const float al = m[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[t] - mx) * a.c2);
+    const float al = m[t] == -INFINITY ? 0.f : pg_ratio<T>(pg_top<T>(m[t], a.c2), mx, a.c2);
     for (int w = 0; w < nw; ++w) {
       if (w == wave) {
 #pragma unroll
@@ -527,7 +542,7 @@ __global__ __launch_bounds__(256, (pg_thin_waves<T, D, NT>())) void paged_thin_k
     const int r = x / (D / N), d = (x - r * (D / N)) * N, i = r / a.group, h = kh * a.group + r - i * a.group;
     float mx = wml[0][r].x, ls = 0.f;
     for (int w = 1; w < nw; ++w) mx = fmaxf(mx, wml[w][r].x);
-    for (int w = 0; w < nw; ++w) ls += pg_share(wml[w][r].y, (wml[w][r].x - mx) * a.c2);
+    for (int w = 0; w < nw; ++w) ls += pg_share<T>(wml[w][r].y, wml[w][r].x, mx, a.c2);
     if (any_bad) ls = NAN;
     float v[N];
 #pragma unroll
@@ -541,7 +556,7 @@ __global__ __launch_bounds__(256, (pg_thin_waves<T, D, NT>())) void paged_thin_k
       const long row = ((long)split * c.tokens + sq.t0 + i) * a.heads + h;
 #pragma unroll
       for (int e = 0; e < N; e += 4) *(f32x4*)(a.part + row * D + d + e) = f32x4{v[e], v[e + 1], v[e + 2], v[e + 3]};
-      if (d == 0) a.ml[row] = float2{any_bad ? 0.f : mx * a.c2, ls};
+      if (d == 0) a.ml[row] = float2{any_bad ? 0.f : mx, ls};
     }
   }
 }
@@ -811,7 +826,7 @@ __global__ __launch_bounds__(64 * NW, (pg_tile_waves<T, D, NW>())) void paged_ti
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
     const float ref = mx == -INFINITY ? 0.f : mx * a.c2;
     if (__any(mx > m)) {
-      const float al = __builtin_amdgcn_exp2f(m * a.c2 - ref);
+      const float al = pg_rescale<T>(m, mx, a.c2, ref);
       l *= al;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) acc[dt] *= al;
@@ -863,7 +878,7 @@ __global__ __launch_bounds__(64 * NW, (pg_tile_waves<T, D, NW>())) void paged_ti
       if (direct) pg_store_row<T, 4>(o + dt * 32 + q * 8, v, a.wide_o);
       else *(f32x4*)(a.part + out_row * D + dt * 32 + q * 8 + 4 * hh) = f32x4{v[0], v[1], v[2], v[3]};
     }
-  if (!direct && hh == 0) a.ml[out_row] = float2{any_bad ? 0.f : m * a.c2, ls};
+  if (!direct && hh == 0) a.ml[out_row] = float2{any_bad ? 0.f : pg_top<T>(m, a.c2), ls};
 }
 
 // ---- joins the splits of a row.  WPR waves of a block of 4 share a (token, head): 1 where rows are many and splits few, 4 where
@@ -896,8 +911,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PgArgs<T> a) {
 #pragma unroll 4
   for (int k = part; k < n; k += WPR) {
     const float2 ml = a.ml[row + k * rows];
-    const float w = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mx);
-    ls += pg_share(ml.y, ml.x - mx);
+    const float w = ml.x == -INFINITY ? 0.f : pg_ratio<T>(ml.x, mx, a.c2);
+    ls += pg_share<T>(ml.y, ml.x, mx, a.c2);
     const float* p = a.part + (row + k * rows) * D + lane * E;
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] += w * p[e];

@@ -928,3 +928,74 @@ def test_c_entries_refuse_shared_memory():
     for table_out, spare_out in ((t + 16, s), (t - 80, s), (t, s + 4), (t, s - 20), (t, t + 92), (s - 92, s), (far, t), (t, far)):
         rc, msg = reorder(t, s, table_out, spare_out)
         assert rc == -1 and "share" in msg, (table_out, spare_out, rc, msg)
+
+
+# ------------------------------------------------------------------------------------------ fp32 sums under a moving maximum
+def _shared_pages(k, v, seqs, page):
+    """one sequence's keys and values [length, heads, dim] as a cache that all of `seqs` sequences read"""
+    length, heads, dim = k.shape
+    per = length // page
+    pages = [x.view(per, page, heads, dim).transpose(1, 2).contiguous().cuda() for x in (k, v)]
+    table = torch.arange(per, dtype=torch.int32).expand(seqs, per).contiguous().cuda()
+    return (*pages, table, torch.full((seqs,), length, dtype=torch.int32).cuda())
+
+
+@gpu
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("n", [12, 32, 40])
+@pytest.mark.parametrize("top", [299.0, 301.0, 407.0])
+def test_fp32_rows_whose_maximum_stands_are_not_rescaled(dim, n, top):
+    """One row of a wave finds a new maximum every 16 keys, the others have the same score everywhere: all their weights are 1,
+    their sums whole numbers, and the half of the values that is 1 gives 1/2 up to the last division (two roundings).  Rows for both
+    forms of the thin kernel and for the tiles; heads and sequences enough that a block has a long run of keys."""
+    length, heads, seqs = 4096, 64, 8
+    k, v = torch.zeros(length, 1, dim), torch.zeros(length, 1, dim)
+    k[:, 0, 0] = (torch.arange(length) // 16).float()
+    k[:, 0, 1] = top
+    v[:length // 2] = 1.0
+    q = torch.zeros(seqs * n, heads, dim)
+    q[:, :, 1] = 1.0
+    q[::n, :, 1], q[::n, :, 0] = 0.0, 1.0
+    args = _shared_pages(k.expand(length, heads, dim), v.expand(length, heads, dim), seqs, 64)
+    out = D.paged_attention(q.cuda(), *args, causal=False, scale=1.0).cpu().view(seqs, n, heads, dim)
+    assert (out[:, 1:] - 0.5).abs().max() <= 2.0 ** -24
+    ref, tol = reference(q[:1, :1], [(k.double(), v.double())], [0], [1], False, 1.0)
+    check(out[:1, 0, :1], ref, tol)
+    assert torch.equal(out[:, 0], out[:1, 0, :1].expand(seqs, heads, dim))
+
+
+@gpu
+@pytest.mark.parametrize("n", [1, 20, 40])
+@pytest.mark.parametrize("top", [299.0, 300.0, 301.0, 407.0, 1000.5])
+def test_fp32_parts_join_by_the_difference_of_their_maxima(n, top):
+    """a long axis in parts, half of them with a maximum one lower than the others': a / (a + b / e).  The lower weight is off by the
+    rounding of c and of the argument (log2 e each, half a step, times ln 2) and a step of the exponential, together 2^-22;
+    the up to 16 parts are added one after the other in numerator and denominator, half a step each, and divided."""
+    length, dim = 4096, 64
+    k, v = torch.zeros(length, 1, dim), torch.zeros(length, 1, dim)
+    k[:, 0, 0] = top - (torch.arange(length) >= length // 2).float()
+    v[:length // 2] = 1.0
+    q = torch.zeros(n, 1, dim)
+    q[:, 0, 0] = 1.0
+    out = D.paged_attention(q.cuda(), *_shared_pages(k, v, 1, 64), causal=False, scale=1.0).cpu().double()
+    want = 1.0 / (1.0 + math.exp(-1.0))
+    assert (out - want).abs().max() <= want * (2.0 ** -22 + 33 * 2.0 ** -24)
+
+
+@gpu
+@pytest.mark.parametrize("n", [32, 64])
+def test_fp32_error_over_a_long_axis_is_that_of_random_roundings(n):
+    """16 384 keys, scores of deviation 2: relative to the output's size the error of a row is, in the mean square, that of independent
+    roundings -- of the dim partial sums of a score (5.5e-7), of the argument's difference, product and constant (2.8, 2.8 and
+    2.4e-7 at 8 below the maximum), of the exponential (0.6e-7) and of some 700 additions to each of two sums (5.4e-7 each):
+    1.1e-6, and at most twice that"""
+    length, heads, seqs, dim = 16384, 32, 16, 128
+    g = torch.Generator().manual_seed(9)
+    k, v = torch.randn(length, heads, dim, generator=g), torch.randn(length, heads, dim, generator=g)
+    q = 2 * torch.randn(seqs * n, heads, dim, generator=g)
+    out = D.paged_attention(q.cuda(), *_shared_pages(k, v, seqs, 64), causal=False).cpu().double()
+    for s, h in ((0, 0), (seqs - 1, heads - 1)):
+        rows = slice(s * n, (s + 1) * n)
+        want = torch.softmax(q[rows, h].double() @ k[:, h].double().t() * dim ** -0.5, -1) @ v[:, h].double()
+        err = (out[rows, h] - want).square().mean(-1).sqrt() / want.square().mean(-1).sqrt()
+        assert err.square().mean().sqrt() <= 2.2e-6, float(err.max())
