@@ -744,8 +744,8 @@ __global__ __launch_bounds__(64 * NW, (pg_tile_waves<T, D, NW>())) void paged_ti
       find_pages(base + 2 * KT < k1 ? base + 2 * KT : k0);
     }
     const char *kt = ksm + buf * KT * ROWB, *vt = vsm + buf * KT * ROWB;
+    bool odd = false;
     if (base + KT > vmin) {                            // some row of the block does not see all of this tile: 0 * inf
-      bool odd = false;
       char* mine = (char*)vt + tid * 16;
 #pragma unroll
       for (int i = 0; i < KT * ROWB / (1024 * NW); ++i) {
@@ -753,7 +753,8 @@ __global__ __launch_bounds__(64 * NW, (pg_tile_waves<T, D, NW>())) void paged_ti
 #pragma unroll
         for (int w = 0; w < 4; ++w) odd |= pg_finite<T>(x[w]) != x[w];
       }
-      if (__syncthreads_or(odd)) {
+      odd = __syncthreads_or(odd);
+      if (odd) {
         // what the infinities and NaN of the tile add to the rows that see them; then they leave the tile
 #pragma unroll 1
         for (int sub = 0; sub < NS; ++sub)
@@ -828,8 +829,10 @@ __global__ __launch_bounds__(64 * NW, (pg_tile_waves<T, D, NW>())) void paged_ti
     if (__any(mx > m)) {
       const float al = pg_rescale<T>(m, mx, a.c2, ref);
       l *= al;
+      // what the tile's infinities have added stays also where what came before goes: by the smallest number there is, not by 0
+      const float keep = odd && al == 0.f ? 0x1p-149f : al;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) acc[dt] *= al;
+      for (int dt = 0; dt < DT; ++dt) acc[dt] *= keep;
       m = mx;
     }
 #pragma unroll

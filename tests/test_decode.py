@@ -999,3 +999,53 @@ def test_fp32_error_over_a_long_axis_is_that_of_random_roundings(n):
         want = torch.softmax(q[rows, h].double() @ k[:, h].double().t() * dim ** -0.5, -1) @ v[:, h].double()
         err = (out[rows, h] - want).square().mean(-1).sqrt() / want.square().mean(-1).sqrt()
         assert err.square().mean().sqrt() <= 2.2e-6, float(err.max())
+
+
+# ------------------------------------------------------------------------------------------- infinite values that a row sees
+def _class(x):
+    return torch.where(torch.isnan(x), 3, torch.where(x == math.inf, 1, torch.where(x == -math.inf, 2, 0)))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("n,length,at", [(3, 3, 1), (50, 50, 2), (50, 50, 40), (300, 300, 5), (300, 300, 200), (50, 1300, 1282),
+                                         (50, 1300, 1260), (50, 1300, 700), (9, 1300, 1294)])
+def test_rows_that_see_an_infinite_value_get_it(dtype, dim, n, length, at):
+    """prompts from their first token on, and the end of a long axis in parts of 256 keys: an infinity in the values goes, with its
+    sign, to the rows that see it (a NaN and infinities of both signs make NaN), and to no other"""
+    pool = Pool([length], 2, dim, 16, dtype, seed=n)
+    k, v = pool.dense[0]
+    q = torch.randn(n, 4, dim, generator=torch.Generator().manual_seed(3)).to(dtype)
+    ref, tol = reference(q, pool.dense, [0], [n], True, dim ** -0.5)
+    for j, row in ((at, [math.inf, -math.inf, math.nan, math.inf]), (at + 1, [0.0, 0.0, 0.0, -math.inf])):
+        pool.v[int(pool.table[0, j // 16]), :, j % 16, 5:9] = torch.tensor(row).to(dtype).cuda()
+    out = D.paged_attention(q.cuda(), *pool.args, max_kv=length).cpu()
+    want = torch.zeros(n, 4, dim, dtype=torch.int64)
+    seen = torch.arange(length - n, length)
+    for col, cls in ((5, 1), (6, 2), (7, 3)):
+        want[seen >= at, :, col] = cls
+    want[seen == at, :, 8], want[seen > at, :, 8] = 1, 3
+    assert torch.equal(_class(out), want)
+    fine = torch.ones(dim, dtype=torch.bool)
+    fine[5:9] = False                                                 # (at + 1 has zeros there now)
+    check(out[:, :, fine], ref[:, :, fine], tol[:, :, fine])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("n", [3, 50])
+def test_infinite_values_where_the_maximum_jumps(dtype, n):
+    """the tile that brings an infinite value raises the maximum so far that what came before weighs nothing: the infinity stays"""
+    dim, length = 64, 64 + n
+    pool = Pool([length], 1, dim, 64, dtype)
+    q = torch.zeros(n, 1, dim, dtype=dtype)
+    q[:, 0, 0] = 1.0
+    page = int(pool.table[0, 1])
+    pool.k[int(pool.table[0, 0]), 0], pool.k[page, 0] = 0.0, 0.0
+    pool.k[page, 0, 0, 0], pool.k[page, 0, 1, 0] = 200.0, 199.0
+    pool.v[page, 0, 1, 9] = math.inf
+    out = D.paged_attention(q.cuda(), *pool.args, scale=1.0).cpu()
+    want = torch.zeros(n, 1, dim, dtype=torch.int64)
+    want[1:, :, 9] = 1                                                # the first of the new tokens does not see it
+    assert torch.equal(_class(out), want)
