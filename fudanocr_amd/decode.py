@@ -280,7 +280,10 @@ class PagedCache:
     lengths and a spare page per sequence.  Every sequence starts with pages of its own.
 
     step (n new tokens for every sequence):  cache.advance(n);  per layer: cache.append(layer, k, v), cache.attend(layer, q);
-    between the steps of a beam search: cache.reorder(parents)."""
+    between the steps of a beam search: cache.reorder(parents).
+
+    A step can be captured into a graph but for `advance`, which counts on the host as well: call it before every replay.  A captured
+    `attend` is sized for max_len, an eager one for the tokens that are there."""
 
     def __init__(self, seqs, max_len, heads, dim, layers=1, page=16, dtype=torch.float32, device="cuda"):
         _need(seqs > 0 and max_len > 0 and heads > 0 and layers > 0, "seqs, max_len, heads and layers must be positive")
@@ -298,16 +301,20 @@ class PagedCache:
 
     def advance(self, n):
         """n more tokens for every sequence (their keys and values follow with `append`)"""
+        _need(not self._captured(), "advance counts on the host: call it before the replay, outside the graph")
         _need(n >= 0 and self.length + n <= self.max_len, "%d + %d tokens in a cache of %d", self.length, n, self.max_len)
         self.length += n
         self.kv_lens += n
+
+    def _captured(self):
+        return self.kv_lens.is_cuda and torch.cuda.is_current_stream_capturing()
 
     def append(self, layer, k_new, v_new):
         paged_append(k_new, v_new, self.k[layer], self.v[layer], self.table, self.kv_lens)
 
     def attend(self, layer, q, causal=True, scale=None, out=None):
         return paged_attention(q, self.k[layer], self.v[layer], self.table, self.kv_lens, causal=causal, scale=scale,
-                               max_kv=self.length, out=out)
+                               max_kv=self.max_len if self._captured() else self.length, out=out)
 
     def reorder(self, parents):
         beam_reorder(parents, self.table, self.kv_lens, self.spare, self.k + self.v, self.table, self.spare)

@@ -1049,3 +1049,51 @@ def test_infinite_values_where_the_maximum_jumps(dtype, n):
     want = torch.zeros(n, 1, dim, dtype=torch.int64)
     want[1:, :, 9] = 1                                                # the first of the new tokens does not see it
     assert torch.equal(_class(out), want)
+
+
+# ------------------------------------------------------------------------------------------------ a cache's step in a graph
+@gpu
+def test_a_captured_step_of_a_cache_replays_as_the_cache_grows():
+    """append, attend and reorder of two layers captured while the cache is nearly empty, replayed to its last token, with eager steps
+    in between, against dense caches; `advance` itself is refused inside the capture"""
+    groups, beams, heads, kv_heads, dim, page, max_len = 2, 3, 4, 2, 64, 8, 300
+    slots = groups * beams
+    g = torch.Generator().manual_seed(12)
+    cache = D.PagedCache(slots, max_len, kv_heads, dim, layers=2, page=page)
+    k, v, q = (torch.zeros(2, slots, h, dim, device="cuda") for h in (kv_heads, kv_heads, heads))
+    parents = torch.zeros(groups, beams, dtype=torch.int32, device="cuda")
+    dense = [[torch.zeros(2, 0, kv_heads, dim, dtype=torch.float64) for _ in range(slots)] for _ in range(2)]
+
+    def step():
+        for layer in range(2):
+            cache.append(layer, k[layer], v[layer])
+        out = [cache.attend(layer, q[layer]) for layer in range(2)]
+        cache.reorder(parents)
+        return out
+    graph = torch.cuda.CUDAGraph()
+    for at in range(max_len):
+        cache.advance(1)
+        new = [torch.randn(2, slots, h, dim, generator=g) for h in (kv_heads, kv_heads, heads)]
+        for dst, src in zip((k, v, q), new):
+            dst.copy_(src)
+        src = torch.randint(0, beams, (groups, beams), generator=g).to(torch.int32)
+        parents.copy_(src)
+        if at == 2:
+            torch.cuda.synchronize()
+            with torch.cuda.graph(graph):
+                _raises("outside the graph", cache.advance, 1)
+                captured = step()
+        if at < 2 or at % 7 == 0:
+            out = step()
+        else:
+            graph.replay()
+            out = captured
+        torch.cuda.synchronize()
+        for layer in range(2):
+            for s in range(slots):
+                dense[layer][s] = torch.cat([dense[layer][s], torch.stack([new[0][layer, s], new[1][layer, s]]).double()[:, None]], 1)
+            if at < 20 or at % 16 in (0, 1) or at > max_len - 3:
+                ref, tol = reference(new[2][layer], dense[layer], list(range(slots)), [1] * slots, True, dim ** -0.5)
+                check(out[layer], ref, tol)
+            dense[layer] = [dense[layer][s // beams * beams + int(src.view(-1)[s])] for s in range(slots)]
+    _raises("in a cache of 300", cache.advance, 1)
