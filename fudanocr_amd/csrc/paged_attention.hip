@@ -44,7 +44,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const char* __restric
   const int s = pg_seq_of_row(c, t, lane);
   const PagedSeq q = paged_seq(c, s);
   const long i = t - q.t0;
-  if (q.bad || i < 0 || i >= q.n) return;
+  if (paged_lost(q) || i < 0 || i >= q.n) return;
   const int pos = q.len - q.n + (int)i;
   if (pos < 0) return;
   const int pg = paged_page(c, s, pos);
@@ -280,7 +280,7 @@ __global__ __launch_bounds__(256, (pg_thin_waves<T, D, NT>())) void paged_thin_k
   const PagedSeq sq = paged_seq(c, s);
   if (sq.n * a.group > a.thin_rows && sq.n <= a.max_q) return;           // the other kernel's
   if (sq.n == 0) return;
-  if (sq.bad || sq.n > a.max_q) {
+  if (paged_lost(sq) || sq.n > a.max_q) {
     if (split == 0 && (sq.n <= a.max_q || a.thin_rows >= a.max_q * a.group)) pg_fill_nan<T, D>(a, sq, kh, 256);
     return;
   }
@@ -621,13 +621,14 @@ __global__ __launch_bounds__(64 * NW, (pg_tile_waves<T, D, NW>())) void paged_ti
     const int* qs = c.q_start;
     const long n = c.per, at = a.tiles - 1 - turn;
     const int grp = a.group;
-    s = pg_find([=](int i) { return paged_first_tile(qs ? qs[i] : i * n, i, grp, ROWS); }, c.seqs, at, lane);
-    tile = (int)(at - paged_first_tile(qs ? qs[s] : s * n, s, grp, ROWS));
+    auto first = [&](int i) { return paged_first_tile(qs ? (long)paged_row(c, qs[i]) : i * n, i, grp, ROWS); };
+    s = pg_find(first, c.seqs, at, lane);
+    tile = (int)(at - first(s));
   }
   const PagedSeq sq = paged_seq(c, s);
   const int R = sq.n * a.group, r0 = tile * ROWS;      // (the host has checked that tokens x heads and a tile more fit)
   if (tile < 0 || r0 >= R || R <= a.thin_rows) return;
-  if (sq.bad || sq.n > a.max_q) {
+  if (paged_lost(sq) || sq.n > a.max_q) {
     if (split == 0)
       for (int x = tid; x < ROWS * D; x += 64 * NW) {
         const int r = r0 + x / D;
@@ -898,7 +899,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PgArgs<T> a) {
   const PagedSeq sq = paged_seq(a.c, s);
   const long i = t - sq.t0;
   const int chunk = sq.n * a.group <= a.thin_rows ? a.chunk : a.tile_chunk;
-  if (i < 0 || i >= sq.n || sq.bad || sq.n > a.max_q || sq.len <= chunk) return;
+  if (i < 0 || i >= sq.n || paged_lost(sq) || sq.n > a.max_q || sq.len <= chunk) return;
   const int n = (paged_visible(sq.len, sq.n, (int)i, a.causal) + chunk - 1) / chunk;
   float mx = -INFINITY;
   for (int k = part * 64 + lane; k < n; k += 64 * WPR) mx = fmaxf(mx, a.ml[row + k * rows].x);

@@ -2,8 +2,9 @@
 // device intrinsics, so that a host program can check every function over whole ranges.
 //
 // Layout: pages [num_pages][heads][page][dim]; row s of `table` names the pages of sequence s in order; kv_lens[s] tokens are
-// in the cache, the new ones included.  All three come from device memory and are not trusted: a sequence whose numbers do
-// not fit is `bad` (its results are NaN, nothing of it is written to the cache) and no address is formed from them.
+// in the cache, the new ones included.  All three, and the rows' offsets, come from device memory and are not trusted: a sequence
+// whose length does not fit is `bad`, one whose rows do not all lie in the tensors `torn` (its results are NaN in the rows that
+// there are, nothing of it is written to the cache) and no address is formed from them.
 #pragma once
 #ifdef __HIPCC__
 #define PG_FN __host__ __device__ __forceinline__
@@ -25,25 +26,33 @@ struct PagedSeq {
   int n;     // how many
   int len;   // tokens in the cache
   bool bad;  // kv_lens[s] out of range
+  bool torn; // its offsets run over the first or the last row
 };
 
-// rows of sequence s: an offset pair that does not lie in order inside [0, tokens] owns no rows
+// an offset as far as it lies in the tensors (which have less than 2^31 rows)
+PG_FN int paged_row(const PagedShape& c, int at) { return at < 0 ? 0 : at > (int)c.tokens ? (int)c.tokens : at; }
+
+// rows of sequence s, as far as they lie in [0, tokens); none where its offsets fall
 PG_FN PagedSeq paged_seq(const PagedShape& c, int s) {
   PagedSeq r;
   if (c.q_start) {
-    const long a = c.q_start[s], b = c.q_start[s + 1];
-    const bool ok = a >= 0 && b >= a && b <= c.tokens;
-    r.t0 = ok ? a : 0;
-    r.n = ok ? (int)(b - a) : 0;
+    const int a = c.q_start[s], b = c.q_start[s + 1], first = paged_row(c, a), rows = paged_row(c, b) - first;
+    r.t0 = first;
+    r.n = rows > 0 ? rows : 0;
+    r.torn = b > a && (unsigned)rows != (unsigned)b - (unsigned)a;
   } else {
     r.n = c.per;
     r.t0 = (long)s * r.n;
+    r.torn = false;
   }
   const int len = c.kv_lens[s];
   r.bad = len < 0 || len > c.max_kv || len > ((long)c.table_ld << c.page_shift);
   r.len = r.bad ? 0 : len;
   return r;
 }
+
+// a sequence that gets NaN for its results and writes nothing
+PG_FN bool paged_lost(const PagedSeq& q) { return q.bad || q.torn; }
 
 // page that holds position pos of sequence s, or -1 when the table names none
 PG_FN int paged_page(const PagedShape& c, int s, int pos) {

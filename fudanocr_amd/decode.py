@@ -13,11 +13,12 @@ A cache is four tensors:
 
 A chunk of new tokens is one packed tensor [tokens, heads, dim]: ``q_start`` (int32 [seqs + 1], non-decreasing) gives the first
 row of every sequence, without it each has tokens / seqs rows.  Rows of no sequence (in front of the first, behind the last)
-are left as they are.  The new tokens of a sequence are its last ones: the first of n has position kv_lens - n.
+are left as they are: in an output that the call allocates they are whatever the memory held.  The new tokens of a sequence are its last ones: the first of n has position kv_lens - n.
 
-What comes from the device is checked there: a length beyond the table or `max_kv`, or more new tokens than `max_q`, makes a
-sequence's output NaN, a page number outside the cache that of the tokens that need the page (other tokens of the sequence
-may be NaN then too); nothing outside the given tensors is read or written."""
+What comes from the device is checked there: a length beyond the table or `max_kv`, more new tokens than `max_q`, or offsets that
+run over the first or the last row make a sequence's output NaN (nothing of it is appended), a page number outside the cache that
+of the tokens that need the page (other tokens of the sequence may be NaN then too); nothing outside the given tensors is read or
+written.  Offsets that fall are not told apart from right ones: rows that two sequences claim may hold either's results, or none."""
 import ctypes
 import math
 

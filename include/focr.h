@@ -480,8 +480,9 @@ int focr_weight_cross_entropy_masked_fwd(const float* logits, const long long* t
  * dtype: 0 fp32, 1 bf16, 2 fp16 -- of q, o, the new keys / values, the pages and the logits; ld* = strides in elements of the
  * token and head axes (rows of dim contiguous).  Pages [num_pages][heads][page][dim], page a power of two 8..1024, dim 64 / 128 /
  * 256; table [seqs][table_ld], kv_lens [seqs] (new tokens included), q_start [seqs + 1] or NULL (tokens / seqs rows each): all
- * int32 in device memory and checked by the kernels -- a sequence whose numbers do not fit gets NaN, nothing outside the given
- * buffers is read or written.  Outputs and pages share no memory with what is read. */
+ * int32 in device memory and checked by the kernels -- a sequence whose length, pages or offsets do not fit gets NaN (where
+ * offsets fall, rows that two sequences claim may hold either's results, or none), nothing outside the given buffers is read or
+ * written.  Outputs and pages share no memory with what is read. */
 #define FOCR_DT_F32 0
 #define FOCR_DT_BF16 1
 #define FOCR_DT_F16 2

@@ -1097,3 +1097,54 @@ def test_a_captured_step_of_a_cache_replays_as_the_cache_grows():
                 check(out[layer], ref, tol)
             dense[layer] = [dense[layer][s // beams * beams + int(src.view(-1)[s])] for s in range(slots)]
     _raises("in a cache of 300", cache.advance, 1)
+
+
+# ------------------------------------------------------------------------------------- offsets that run over the rows there are
+def test_offsets_that_do_not_fit_on_the_cpu(tmp_path):
+    """csrc/paged_index.h on offsets in front of the first row and behind the last, under sanitizers (tests/cpp/paged_offsets_check.cpp)"""
+    exe = str(tmp_path / "paged_offsets_check")
+    subprocess.check_call(["g++", "-std=c++17", "-O1", "-g", "-fsanitize=address,undefined", "-fno-sanitize-recover=all", "-I",
+                           os.path.join(ROOT, "fudanocr_amd", "csrc"), os.path.join(ROOT, "tests", "cpp", "paged_offsets_check.cpp"),
+                           "-o", exe])
+    out = subprocess.run([exe], capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and out.stdout.startswith("ok"), out.stdout[-2000:] + out.stderr[-2000:]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("seqs", [3, 64, 65, 150])
+@pytest.mark.parametrize("news", [1, 7, 90])
+@pytest.mark.parametrize("heads", [2, 8])
+def test_offsets_over_the_first_and_last_row_give_nan(dtype, seqs, news, heads):
+    """the first sequence claims rows in front of the tensor, the last ones rows behind it: NaN in the rows of theirs that there are,
+    the others' results as they would be, and an append that writes the others' rows alone"""
+    lens = [news + 30] * seqs
+    pool = Pool(lens, 2, 64, 16, dtype)
+    starts = [i * news for i in range(seqs + 1)]
+    tokens = starts[seqs - 1] + (news + 1) // 2                       # half of the last sequence is there
+    g = torch.Generator().manual_seed(4)
+    q = torch.randn(tokens, heads, 64, generator=g).to(dtype)
+    ref, tol = reference(q, pool.dense[1:-1], starts[1:-2], [news] * (seqs - 2), True, 0.125)
+    for over in (1, 1000, 2 ** 31 - 1 - starts[-1]):
+        qs = torch.tensor(starts, dtype=torch.int32)
+        qs[0] = -over
+        qs[-1] += over
+        for kw in ({}, {"max_q": news + 1000, "max_kv": news + 30}):
+            out = torch.full((tokens, heads, 64), 7.0, dtype=dtype, device="cuda")
+            D.paged_attention(q.cuda(), *pool.args, q_start=qs.cuda(), out=out, **kw)
+            assert torch.isnan(out[:news]).all() and torch.isnan(out[starts[-2]:]).all()
+            check(out[starts[1]:starts[-2]], ref[starts[1]:starts[-2]], tol[starts[1]:starts[-2]])
+    qs[-2] = 2 ** 31 - 2                                              # the last sequence has no rows, the one before it too many
+    out = D.paged_attention(q.cuda(), *pool.args, q_start=qs.cuda())
+    assert torch.isnan(out[:news]).all() and torch.isnan(out[starts[-3]:]).all()
+    check(out[starts[1]:starts[-3]], ref[starts[1]:starts[-3]], tol[starts[1]:starts[-3]])
+    before = pool.k.clone()
+    new = torch.full((tokens, 2, 64), 3.0, dtype=dtype, device="cuda")
+    D.paged_append(new, new, *pool.args[:2], *pool.args[2:], q_start=qs.cuda())
+    for s in range(seqs):
+        pages = [int(pool.table[s, j]) for j in range(-(-lens[s] // 16))]
+        now, was = (torch.cat([x[p] for p in pages], 1)[:, :lens[s]] for x in (pool.k, before))
+        if 0 < s < seqs - 2:
+            assert (now[:, 30:] == 3).all() and torch.equal(now[:, :30], was[:, :30])
+        else:
+            assert torch.equal(now, was)
