@@ -118,5 +118,5 @@ class Transformer(nn.Module):
         """the `beams` most likely strings of every image: (tokens int64 [B, beams, max_len], log-probabilities fp32 [B, beams]),
         best first, closed with '-' (fudanocr_amd/sld/beam.py).  image NCHW [B,1,32,128]; eval mode."""
         from ..sld import beam
-        return beam.search(self, lambda: self.encoder(image), self.embedding_word, self.generator_word, beams, max_len,
-                           alphabet.index("-"), alphabet.index("-"))
+        return beam.search(self, image.shape[0], lambda: self.encoder(image), self.embedding_word, self.generator_word, beams,
+                           max_len, alphabet.index("-"), alphabet.index("-"))

@@ -79,5 +79,5 @@ class Transformer(nn.Module):
 
         def encode():
             return self.encoder(K.bicubic_gray(image, image.shape[3]) if image.shape[1] == 4 else image)
-        return beam.search(self, encode, self.embedding_word_with_upperword, self.generator_word_with_upperword, beams, max_len,
-                           alphabet.index("0"), alphabet.index("0"))
+        return beam.search(self, image.shape[0], encode, self.embedding_word_with_upperword, self.generator_word_with_upperword,
+                           beams, max_len, alphabet.index("0"), alphabet.index("0"))

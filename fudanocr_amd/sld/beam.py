@@ -17,21 +17,23 @@ def _norm(ln, x, residual):
 
 
 @torch.no_grad()
-def search(model, encode, embedding, generator, beams, max_len, start, eos):
-    """encode() -> the encoder's output NHWC [B, H, W, 1024], called once the arguments are checked -> (tokens
-    int64 [B, beams, max_len], scores fp32 [B, beams]), best first.  A hypothesis ends with its first `eos`; the positions behind
-    it hold `eos` too.  Nothing in here waits for the device."""
+def search(model, batch, encode, embedding, generator, beams, max_len, start, eos):
+    """encode() -> the encoder's output NHWC [batch, H, W, 1024], called once the arguments are checked -> (tokens
+    int64 [batch, beams, max_len], scores fp32 [batch, beams]), best first.  A hypothesis ends with its first `eos`; the
+    positions behind it hold `eos` too.  Nothing in here waits for the device."""
     if model.training:
         raise RuntimeError("beam_search needs the model in eval mode")
     if not (1 <= beams <= 64 and max_len >= 1 and max_len <= model.pe.pe.shape[1]):
         raise RuntimeError("beam_search: beams must be 1 to 64, max_len 1 to %d" % model.pe.pe.shape[1])
+    if batch * beams > 65535 and max_len > 1:               # (a single step reorders nothing)
+        raise RuntimeError("beam_search: batch x beams must be at most 65535, got %d x %d" % (batch, beams))
     vocab = generator.proj.weight.shape[0]
     if not (0 <= start < vocab and 0 <= eos < vocab):
         raise RuntimeError("beam_search: start and eos must be inside the %d classes" % vocab)
     feat = encode()
     dec, dev = model.decoder, feat.device
     own, cross = dec.mask_multihead, dec.multihead
-    batch, hh, ww, dm = feat.shape
+    _, hh, ww, dm = feat.shape
     slots = batch * beams
     if batch == 0:
         return torch.empty((0, beams, max_len), dtype=torch.int64, device=dev), torch.empty((0, beams), device=dev)

@@ -259,5 +259,6 @@ class Transformer(nn.Module):
 
         def encode():
             return self.encoder(K.to_nhwc(image)) if conv_feature is None else K.to_nhwc(conv_feature)
-        return beam.search(self, encode, self.embedding_word, self.generator_word, beams, max_len, alphabet.index("<"),
+        batch = (image if conv_feature is None else conv_feature).shape[0]
+        return beam.search(self, batch, encode, self.embedding_word, self.generator_word, beams, max_len, alphabet.index("<"),
                            alphabet.index("$"))

@@ -1148,3 +1148,19 @@ def test_offsets_over_the_first_and_last_row_give_nan(dtype, seqs, news, heads):
             assert (now[:, 30:] == 3).all() and torch.equal(now[:, :30], was[:, :30])
         else:
             assert torch.equal(now, was)
+
+
+def test_beam_search_refuses_more_beams_than_a_reorder_takes():
+    """batch x beams over 65 535 is refused before the encoder runs, not by the first step's reorder"""
+    from fudanocr_amd.loss.transformer import Transformer as Characters
+    from fudanocr_amd.loss.transformer_english_decomposition import Transformer as EnglishStrokes
+    from fudanocr_amd.sld.model.transformer import Transformer as Strokes
+
+    def never(*a, **kw):
+        raise AssertionError("the encoder ran")
+    for model, shape in ((Strokes("stroke"), (3, 32, 32)), (Characters(), (1, 32, 128)), (EnglishStrokes(), (4, 32, 128))):
+        model.encoder.forward = never
+        image = torch.zeros(1, *shape).expand(1024, *shape)
+        _raises("65535", model.eval().beam_search, image, beams=64)
+        _raises("65535", model.beam_search, torch.zeros(1, *shape).expand(65536, *shape), beams=1)
+    _raises("65535", Strokes("stroke").eval().beam_search, None, beams=64, conv_feature=torch.zeros(1, 1, 1, 1).expand(1024, 1024, 8, 8))
