@@ -21,11 +21,11 @@
 //     they are appended to a buffer by ballot, as 64-bit keys (the value's bits in an order that compares as integers, then the
 //     complement of the index), and put in order at the end.  (A bound that grows with the chunks, candidates taken from
 //     the registers: 45 us at 64 x 8 x 50001 where this takes 36.)  Rows of nearly one value -- a vocabulary masked to a few
-//     tokens -- have all lanes read again, in order: 64 us at that size.
+//     tokens -- have all lanes read again, in order: 62 us at that size (fp32 79, where other rows take 38).
 // Segments start at fixed indices and lanes take fixed indices of them whatever the row's alignment, so equal rows have
 // equal sums.  A second pass over K x segments lists of n joins them (in the same block where a batch entry is small).
-// Measured (64 entries x 8 beams x 50001, bf16, 51 MB): scan 29 us -- 12 for the loads alone, 12 more for the exponentials, 5 for
-// the candidates -- and 7 us for the join.
+// Measured (64 entries x 8 beams x 50001, bf16, 51 MB): scan 27 us -- 12 for the loads alone, 12 more for the exponentials, the rest
+// for the candidates -- and 7 us for the join; 33 us a call.
 #define BS_CHUNK 2048
 #define BS_MAX 64                     // beams, and candidates asked for
 #define BS_WAVES 16                   // of the one-launch form
@@ -436,8 +436,9 @@ __global__ __launch_bounds__(64 * BS_WAVES) void beam_join_kernel(BsArgs a, int 
 }
 
 // One launch with a block per batch entry while an entry has at most 16 K logits; else the rows are cut into segments of whole
-// chunks, about 2048 waves in all (64 x 8 x 50001 bf16: 36 us, twice as many 39), and joined by a second
-// launch (64 x 5 x 6625 fp32: 18.7 us, in one launch 21.5, both with a slower join).
+// chunks, about 2048 waves in all (64 x 8 x 50001 bf16: 33 us, twice as many 36.5), and joined by a second launch.  A call of 64
+// entries x 5 beams, fp32, in one / two launches: 2000 classes 10.9 / 14.7 us, 3270 (16 K logits) 13.4 / 14.6, 4500 15.3 / 14.4, 6625
+// 16.9 / 14.6; of 1 and 16 entries the same within 1 us, of 128 at 6625 both 17.5.
 struct BsPlan {
   bool one;
   int parts, seg;
@@ -498,7 +499,8 @@ extern "C" int focr_beam_select(const void* logits, long ldb, long ldk, const fl
 // written again, so j takes p's table entries for them.  The last, partial page (L % page tokens) will be written by every
 // beam: a j != p gets its own copy, in its spare page, and the page it held before becomes its spare.  So a beam moves at most
 // page - 1 tokens however long the sequence, and no page is allocated or freed.  Bound by the bytes moved: 64 x 8 beams, 4 layers of
-// 8 x 128 bf16, pages of 64: 97 us for 205 MB written and as many read, in pieces of 8 KB (a large copy: 4.9 TB/s, this 4.2).
+// 8 x 128 bf16, pages of 64: 87 us for 209 MB written and as many read, in runs of 8 KB (4.8 TB/s; a large copy: 4.9), a call
+// 94 .. 102 us.
 // ======================================================================================================================
 #define BR_MAX_TENSORS 64
 #define BR_PIECE 1024                 // 16-byte units a block moves (512 .. 2048: 97 .. 110 us)

@@ -251,8 +251,9 @@ __device__ __forceinline__ void pg_fill_nan(const PgArgs<T>& a, const PagedSeq& 
 //                 registers (v_perm, 16-bit types; a choice of registers in fp32); tile (u, c) of O^T then has row e <-> d =
 //                 16 CH u + CH e + c.
 // The next tile's loads go out between the two products.  MFMA time is a tenth of the bytes' (16-bit) to a third (fp32).
-// Measured: 64 sequences of 100 .. 8190 tokens, 8 key heads x 128 bf16: 178 us = 5.5 TB/s; two of 131 000: 183 us = 5.8 TB/s; 128
-// images x 256 positions, 16 heads x 64 fp32: 42 us = 6.3 TB/s (a large copy on this card: 4.9 TB/s read and written).
+// Measured: 64 sequences of 100 .. 8190 tokens, 8 key heads x 128 bf16: 173 us = 5.7 TB/s; two of 131 000: 177 us = 6.1 TB/s; 128
+// images x 256 positions, 16 heads x 64 fp32: 43 us = 6.4 TB/s (a large copy on this card: 4.9 TB/s read and written).  32 rows a key
+// head (32 sequences x 4 tokens over 4000, 4 key heads x 128), per call: bf16 61 us = 4.3 TB/s, fp32 131 us = 4.0.
 // ======================================================================================================================
 #define PG_MAX_CHUNK 8192
 // Queries that take 32 registers or more go through LDS.  At most 256 registers keep two waves on a SIMD; 16-bit rows of 256
@@ -568,9 +569,10 @@ __global__ __launch_bounds__(256, (pg_thin_waves<T, D, NT>())) void paged_thin_k
 // KT keys and values at a time in LDS, double-buffered by direct loads, 16-byte chunks XOR-swizzled by row so that both the
 // row-wise reads of K and the transposing reads of V (ds_read_b64_tr_b16; plain words in fp32) use every bank.  A wave skips
 // the tiles that none of its rows sees and compares positions only where its rows differ.
-// Measured: 4096 tokens after 12288, 32 heads over 8, 128 bf16: 0.95 ms = 1010 TFLOP/s, where a large library product of the same
-// type reaches 1104; the matrix pipe is 0.46 busy and the vector pipe (the exponentials, above all) 0.52: two waves a SIMD run as
-// the sum of the two.  fp32 rows of 128: 110 TFLOP/s on the exact instructions (library product: 151).
+// Measured: 4096 tokens after 12288, 32 heads over 8, 128 bf16: 0.96 ms = 1000 TFLOP/s (0.97 .. 1.0 ms a call, box to box), where a
+// large library product of the same type reaches 1104; the matrix pipe is 0.45 busy and the vector pipe (the exponentials, above all)
+// 0.52: two waves a SIMD run as the sum of the two.  fp32 rows of 64 / 128 / 256: 86 / 111 / 82 TFLOP/s on the exact instructions
+// (library product: 151); fp16 rows of 64: 592, bf16 rows of 256, which spill: 521.
 // ======================================================================================================================
 template <int CPR> __device__ __forceinline__ int pg_swz(int row) {
   if constexpr (CPR == 8) return ((row >> 1 & 1) << 2) | ((row >> 2 & 1) << 1) | (row >> 3 & 1);
@@ -599,8 +601,8 @@ __global__ __launch_bounds__(64 * NW, (pg_tile_waves<T, D, NW>())) void paged_ti
   const int kh = blockIdx.x % a.kv_heads, split = blockIdx.x / a.kv_heads / a.tiles;
   const int turn = blockIdx.x / a.kv_heads % a.tiles;
   // The tiles with the most keys first, so that the last blocks to finish are short ones.  Up to 64 sequences are put in order of
-  // their lengths by the wave itself (24 chunks of 1 .. 764 tokens behind 300 .. 4000: 216 us in the order of the rows, 205 us
-  // so); more of them fill the card well enough from the last row to the first.
+  // their lengths by the wave itself (24 chunks of 1 .. 764 tokens behind 300 .. 4000: 205 us so, 216 us in the order of the rows;
+  // with the priorities below 188); more of them fill the card well enough from the last row to the first.
   int s, tile;
   if (c.seqs <= 64) {
     int len = 0, mine = 0, start = 0;
@@ -810,7 +812,7 @@ __global__ __launch_bounds__(64 * NW, (pg_tile_waves<T, D, NW>())) void paged_ti
       }
     }
     // The softmax of one wave ahead of the products of its neighbour on the SIMD, while two blocks of 4 waves share a CU (the 24
-    // chunks: 204 -> 187 us); in one block of 8 it costs 2 %
+    // chunks: 204 -> 188 us); in one block of 8 it costs 2 %
     if constexpr (NW == 4) __builtin_amdgcn_s_setprio(1);
     if (base + KT > wvmin) {
 #pragma unroll
@@ -981,7 +983,8 @@ extern "C" int focr_paged_append(const void* k_new, const void* v_new, long ldtk
 }
 
 // Splits of the key axis.  The keys of a (sequence, key head) go to blocks of `chunk` keys; a sequence of at most `chunk` keys
-// writes its output directly, the parts of a longer one are joined by a second launch.  Up to 4096 blocks, so that sequences
+// writes its output directly, the parts of a longer one are joined by a second launch.  (Times here compare the forms as they were
+// when the rule was made.)  Up to 4096 blocks, so that sequences
 // of very different lengths still fill the card evenly (64 sequences of 100 .. 8190 tokens x 8 heads, bf16, 128 wide: 2048
 // blocks 198 us, 4096 193 us, 8192 200 us), but no fewer than 1024 keys in a block while there are blocks enough for two on each
 // CU: a block's start and end cost as much as some hundred keys (2 sequences of 131k: 1024 keys 205 us, 512 224 us, 256 254 us).

@@ -133,7 +133,7 @@ def paged_attention(q, k_pages, v_pages, table, kv_lens, q_start=None, causal=Tr
     """softmax(scale q k^T) v of the new tokens q [tokens, heads, dim] over their sequences' caches -> [tokens, heads, dim].
 
     heads is a multiple of the cache's; head h reads the cache's head h // (heads / cache heads).  causal: a token at position p
-    sees the positions 0 .. p, else all kv_lens of them; a token that sees nothing gets zeros.  scale: 1 / sqrt(dim) unless
+    sees the positions 0 .. p, else all kv_lens of them; a token that sees nothing, or scores of -inf alone, gets zeros.  scale: 1 / sqrt(dim) unless
     given, positive.  max_q / max_kv: bounds on a sequence's new tokens and on kv_lens that the caller knows (they size the
     launch; the defaults are the most the tensors allow).  out: where to write (apart from q and the cache)."""
     num_pages, kv_heads, page, dim, seqs, ld, dt, dev = _cache(k_pages, v_pages, table, kv_lens, q_start)
