@@ -13,7 +13,8 @@ A cache is four tensors:
 
 A chunk of new tokens is one packed tensor [tokens, heads, dim]: ``q_start`` (int32 [seqs + 1], non-decreasing) gives the first
 row of every sequence, without it each has tokens / seqs rows.  Rows of no sequence (in front of the first, behind the last)
-are left as they are: in an output that the call allocates they are whatever the memory held.  The new tokens of a sequence are its last ones: the first of n has position kv_lens - n.
+are left as they are: in an output that the call allocates they are whatever the memory held.  The new tokens of a sequence are
+its last ones: the first of n has position kv_lens - n.
 
 What comes from the device is checked there: a length beyond the table or `max_kv`, more new tokens than `max_q`, or offsets that
 run over the first or the last row make a sequence's output NaN (nothing of it is appended), a page number outside the cache that
@@ -133,9 +134,9 @@ def paged_attention(q, k_pages, v_pages, table, kv_lens, q_start=None, causal=Tr
     """softmax(scale q k^T) v of the new tokens q [tokens, heads, dim] over their sequences' caches -> [tokens, heads, dim].
 
     heads is a multiple of the cache's; head h reads the cache's head h // (heads / cache heads).  causal: a token at position p
-    sees the positions 0 .. p, else all kv_lens of them; a token that sees nothing, or scores of -inf alone, gets zeros.  scale: 1 / sqrt(dim) unless
-    given, positive.  max_q / max_kv: bounds on a sequence's new tokens and on kv_lens that the caller knows (they size the
-    launch; the defaults are the most the tensors allow).  out: where to write (apart from q and the cache)."""
+    sees the positions 0 .. p, else all kv_lens of them; a token that sees nothing, or scores of -inf alone, gets zeros.  scale:
+    1 / sqrt(dim) unless given, positive.  max_q / max_kv: bounds on a sequence's new tokens and on kv_lens that the caller knows
+    (they size the launch; the defaults are the most the tensors allow).  out: where to write (apart from q and the cache)."""
     num_pages, kv_heads, page, dim, seqs, ld, dt, dev = _cache(k_pages, v_pages, table, kv_lens, q_start)
     tokens, heads, qt, qh = _rows(q, None, dim, dt, dev, "q")
     _need(heads > 0 and heads % kv_heads == 0, "%d heads over a cache of %d", heads, kv_heads)
@@ -283,8 +284,8 @@ class PagedCache:
     step (n new tokens for every sequence):  cache.advance(n);  per layer: cache.append(layer, k, v), cache.attend(layer, q);
     between the steps of a beam search: cache.reorder(parents).
 
-    A step can be captured into a graph but for `advance`, which counts on the host as well: call it before every replay.  A captured
-    `attend` is sized for max_len, an eager one for the tokens that are there."""
+    A step can be captured into a graph but for `advance`, which counts on the host as well: call it before every replay.  A
+    captured `attend` is sized for max_len, an eager one for the tokens that are there."""
 
     def __init__(self, seqs, max_len, heads, dim, layers=1, page=16, dtype=torch.float32, device="cuda"):
         _need(seqs > 0 and max_len > 0 and heads > 0 and layers > 0, "seqs, max_len, heads and layers must be positive")
